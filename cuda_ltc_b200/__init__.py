@@ -7,8 +7,13 @@ from . import _lib  # noqa: F401
 from .api import (  # noqa: F401
     Context,
     HostStepPipeline,
+    Kv8Cache,
     LtcaError,
     attention_backward,
     attention_decode,
     attention_forward,
+    kv8_append,
+    kv8_decode,
+    kv8_read,
+    kv8_select,
 )

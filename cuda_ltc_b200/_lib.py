@@ -70,6 +70,55 @@ class TsaParams(C.Structure):
     ]
 
 
+class Kv8CacheParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("S", C.c_int32), ("D", C.c_int32), ("block", C.c_int32),
+        ("k", C.c_void_p), ("k_strides", Strides),
+        ("v", C.c_void_p), ("v_strides", Strides),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("bounds", C.c_void_p),
+    ]
+
+
+class Kv8AppendParams(C.Structure):
+    _fields_ = [
+        ("n", C.c_int32), ("dtype", C.c_int32),
+        ("k", C.c_void_p), ("k_strides", Strides),
+        ("v", C.c_void_p), ("v_strides", Strides),
+        ("kv_len", C.c_void_p), ("new_len", C.c_void_p),
+    ]
+
+
+class Kv8ReadParams(C.Structure):
+    _fields_ = [
+        ("start", C.c_int32), ("n", C.c_int32), ("dtype", C.c_int32),
+        ("k", C.c_void_p), ("k_strides", Strides),
+        ("v", C.c_void_p), ("v_strides", Strides),
+        ("kv_len", C.c_void_p),
+    ]
+
+
+class Kv8DecodeParams(C.Structure):
+    _fields_ = [
+        ("Hq", C.c_int32), ("Sq", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
+        ("scale", C.c_float), ("score_clamp", C.c_float),
+        ("q", C.c_void_p), ("q_strides", Strides),
+        ("o", C.c_void_p), ("o_strides", Strides),
+        ("lse", C.c_void_p), ("keep_mask", C.c_void_p), ("kv_len", C.c_void_p), ("new_len", C.c_void_p),
+        ("blocks", C.c_void_p), ("n_blocks", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class Kv8SelectParams(C.Structure):
+    _fields_ = [
+        ("Hq", C.c_int32), ("Sq", C.c_int32), ("dtype", C.c_int32),
+        ("q", C.c_void_p), ("q_strides", Strides),
+        ("kv_len", C.c_void_p), ("new_len", C.c_void_p),
+        ("first", C.c_int32), ("last", C.c_int32), ("count", C.c_int32),
+        ("blocks", C.c_void_p),
+    ]
+
+
 # Every symbol include/ltc_attn.h declares, with its ctypes signature.
 EXPORTS = {
     "ltca_version": (C.c_int, []),
@@ -89,6 +138,12 @@ EXPORTS = {
     "ltca_attn_decode": (C.c_int, [C.c_void_p, C.POINTER(AttnParams)]),
     "ltca_attn_decode_workspace_bytes": (C.c_int, [C.POINTER(AttnParams), C.POINTER(C.c_size_t)]),
     "ltca_attn_decode_static": (C.c_int, [C.c_void_p, C.POINTER(AttnParams), C.c_char_p, C.c_size_t]),
+    "ltca_kv8_append": (C.c_int, [C.c_void_p, C.POINTER(Kv8CacheParams), C.POINTER(Kv8AppendParams)]),
+    "ltca_kv8_read": (C.c_int, [C.c_void_p, C.POINTER(Kv8CacheParams), C.POINTER(Kv8ReadParams)]),
+    "ltca_kv8_decode": (C.c_int, [C.c_void_p, C.POINTER(Kv8CacheParams), C.POINTER(Kv8DecodeParams)]),
+    "ltca_kv8_decode_workspace_bytes": (C.c_int, [C.POINTER(Kv8CacheParams), C.POINTER(Kv8DecodeParams),
+                                                  C.POINTER(C.c_size_t)]),
+    "ltca_kv8_select": (C.c_int, [C.c_void_p, C.POINTER(Kv8CacheParams), C.POINTER(Kv8SelectParams)]),
     "ltca_tsa_bwd": (C.c_int, [C.c_void_p, C.POINTER(TsaParams)]),
     "ltca_tsa_saved_bytes": (C.c_int, [C.POINTER(TsaParams), C.POINTER(C.c_size_t)]),
     "ltca_tsa_weight_cache_bytes": (C.c_int, [C.POINTER(TsaParams), C.POINTER(C.c_size_t)]),

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -40,6 +40,17 @@ def _strides(t: torch.Tensor) -> Strides:
     return Strides(t.stride(0), t.stride(1), t.stride(2))
 
 
+class Kv8Cache(NamedTuple):
+    """Keys and values in e4m3 with a power-of-two scale for each block of tokens and head (``ltca_kv8_cache``):
+    value = code * scale.  Any strides of k and v with head_dim contiguous and rows on 16-byte boundaries will do."""
+    k: torch.Tensor                     # float8_e4m3fn [batch, heads, capacity, head_dim]
+    v: torch.Tensor
+    k_scale: torch.Tensor               # float32 [batch, heads, ceil(capacity / block)]
+    v_scale: torch.Tensor
+    bounds: Optional[torch.Tensor]      # int8 [batch, heads, ceil(capacity / block), 2, head_dim], for kv8_select
+    block: int                          # tokens that share a scale: 16, 32, 64 or 128
+
+
 class Context:
     """One (device, stream) binding of the library."""
 
@@ -53,7 +64,7 @@ class Context:
         if rc != 0:
             raise LtcaError(rc, "ltca_ctx_create failed (is this an sm_100 GPU?)")
         self.handle = handle
-        self._host = _lib.load_host(LtcaError).Host(handle.value, self.device)
+        self._host = _lib.load_host(LtcaError).Host(handle.value, self.device, sptr.value or 0)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -68,7 +79,7 @@ class Context:
             pass
 
     def set_stream(self, stream: torch.cuda.Stream):
-        self.lib.ltca_ctx_set_stream(self.handle, C.c_void_p(stream.cuda_stream))
+        self._host.set_stream(stream.cuda_stream)
 
     def enable_kernel_timing(self, enable: bool = True):
         """Per-kernel CUDA-event timing of the tensor-pipe backward (benchmark aid)."""
@@ -183,6 +194,37 @@ class Context:
     def attn_decode(self, q, k, v, kv_len=None, scale=None, keep_mask=None, score_clamp=0.0,
                     out=None, lse=None):
         return self._host.attn_decode(q, k, v, kv_len, scale, keep_mask, score_clamp, out, lse)
+
+    # ---- 8-bit key/value cache -----------------------------------------------------------
+    def kv8_cache(self, B, H, capacity, D, block=64, bounds=False) -> Kv8Cache:
+        """An empty cache for B sequences of up to ``capacity`` tokens; ``bounds=True`` for one that kv8_select is called on."""
+        dev = torch.device("cuda", self.device)
+        nb = -(-capacity // block)
+        k, v = (torch.zeros((B, H, capacity, D), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.ones((B, H, nb), dtype=torch.float32, device=dev) for _ in range(2))
+        return Kv8Cache(k, v, ks, vs, torch.zeros((B, H, nb, 2, D), dtype=torch.int8, device=dev) if bounds else None, block)
+
+    def kv8_append(self, cache, k, v, kv_len, new_len=None):
+        """Quantises new keys and values [B, H, n, D] into the cache at positions kv_len - new_len on, where ``kv_len`` (int32
+        [B]) counts the new tokens already and ``new_len`` (int32 [B], default n) says how many of the n each sequence has."""
+        self._host.kv8_append(cache, k, v, kv_len, new_len)
+
+    def kv8_read(self, cache, kv_len=None, start=0, count=None, dtype=None, out_k=None, out_v=None):
+        """k, v [B, H, count, D] of positions ``start`` on, in bfloat16 or float32 (``dtype``, else out_k's, else bfloat16);
+        zeros from kv_len on."""
+        return self._host.kv8_read(cache, kv_len, start, count, dtype, out_k, out_v)
+
+    def kv8_decode(self, q, cache, kv_len=None, new_len=None, scale=None, causal=True, keep_mask=None, score_clamp=0.0,
+                   blocks=None, out=None, lse=None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """out, lse of the newest tokens' queries [B, Hq, Sq, D] over the cache; heads of queries share heads of keys where there
+        are more of them.  Query i of a sequence stands at kv_len - new_len + i (``new_len`` int32 [B], default Sq; rows behind
+        it are zero).  ``blocks`` (int32 [B, H, n], as kv8_select gives them): only keys of these blocks of tokens."""
+        return self._host.kv8_decode(q, cache, kv_len, new_len, scale, causal, keep_mask, score_clamp, blocks, out, lse)
+
+    def kv8_select(self, q, cache, kv_len, count, new_len=None, first=1, last=1, out=None) -> torch.Tensor:
+        """int32 [B, H, count]: the blocks of tokens whose bounds allow the largest products with the queries, the ``first``
+        and the ``last`` live ones always among them; rising, -1 behind the last."""
+        return self._host.kv8_select(q, cache, kv_len, count, new_len, first, last, out)
 
     # ---- sequence sharding: fold one key/value shard's result into running accumulators ----
     def attn_merge(self, o_acc, lse_acc, o_blk, lse_blk, s0=0):
@@ -353,3 +395,23 @@ def attention_backward(q, k, v, o, lse, dout, **kw):
 def attention_decode(q, k, v, kv_len=None, **kw):
     """Single-query step over a key/value cache.  See :meth:`Context.attn_decode`."""
     return _ctx_for(q).attn_decode(q, k, v, kv_len=kv_len, **kw)
+
+
+def kv8_append(cache, k, v, kv_len, **kw):
+    """New keys and values into an 8-bit cache.  See :meth:`Context.kv8_append`."""
+    _ctx_for(k).kv8_append(cache, k, v, kv_len, **kw)
+
+
+def kv8_read(cache, **kw):
+    """An 8-bit cache's keys and values in fp32 or bf16.  See :meth:`Context.kv8_read`."""
+    return _ctx_for(cache[0]).kv8_read(cache, **kw)
+
+
+def kv8_decode(q, cache, kv_len=None, **kw):
+    """Attention of the newest tokens over an 8-bit cache.  See :meth:`Context.kv8_decode`."""
+    return _ctx_for(q).kv8_decode(q, cache, kv_len=kv_len, **kw)
+
+
+def kv8_select(q, cache, kv_len, count, **kw):
+    """The blocks of an 8-bit cache that the newest tokens should read.  See :meth:`Context.kv8_select`."""
+    return _ctx_for(q).kv8_select(q, cache, kv_len, count, **kw)

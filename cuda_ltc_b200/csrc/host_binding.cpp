@@ -14,6 +14,9 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -41,6 +44,7 @@ struct Host {
     PyObject_HEAD
     ltca_ctx* ctx;
     int device;
+    cudaStream_t stream; // the context's
     at::Tensor* ws;      // scratch, grown on demand and kept
 };
 
@@ -262,6 +266,210 @@ PyObject* attn_bwd(Host* h, PyObject* const* a) {
     return Py_BuildValue("NNN", result(a[12], g[0]), result(a[13], g[1]), result(a[14], g[2]));
 }
 
+// ---- the 8-bit key/value cache -------------------------------------------------------------------
+inline void on_device(const Host* h, const at::Tensor& t, const char* msg) {
+    require(t.is_cuda() && t.device().index() == (c10::DeviceIndex)h->device, msg);
+}
+int float_type(at::ScalarType t) {
+    if (t == at::kFloat) return LTCA_F32;
+    if (t == at::kBFloat16) return LTCA_BF16;
+    raise(PyExc_TypeError, "unsupported dtype: the tensors must be float32 or bfloat16");
+}
+inline int int32_of(PyObject* o, const char* msg) {
+    const int64_t v = integer(o);
+    require(v >= INT32_MIN && v <= INT32_MAX, msg);
+    return (int)v;
+}
+
+// cache: (k, v, k_scale, v_scale, bounds or None, block)
+void fill_cache(const Host* h, ltca_kv8_cache& c, PyObject* cache) {
+    std::memset(&c, 0, sizeof(c));
+    if (!PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != 6)
+        raise(PyExc_TypeError, "a cache is a tuple (k, v, k_scale, v_scale, bounds, block): Context.kv8_cache makes one");
+    const at::Tensor& k = tensor(PyTuple_GET_ITEM(cache, 0));
+    const at::Tensor& v = tensor(PyTuple_GET_ITEM(cache, 1));
+    on_device(h, k, "the cache must be on the context's device");
+    on_device(h, v, "the cache must be on the context's device");
+    require(k.dim() == 4 && k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn,
+            "the cache's k and v are float8_e4m3fn [batch, heads, capacity, head_dim]");
+    for (int i = 0; i < 4; ++i) require(k.size(i) <= INT32_MAX, "the cache is too large");
+    same_shape(v, k.size(0), k.size(1), k.size(2), k.size(3), "the cache's v must have the shape of its k");
+    c.B = (int32_t)k.size(0); c.H = (int32_t)k.size(1); c.S = (int32_t)k.size(2); c.D = (int32_t)k.size(3);
+    c.block = int32_of(PyTuple_GET_ITEM(cache, 5), "bad block");
+    c.k = k.data_ptr(); c.k_strides = strides(k);
+    c.v = v.data_ptr(); c.v_strides = strides(v);
+    require(c.block >= 1, "bad block");
+    const int64_t nb = (k.size(2) + c.block - 1) / c.block;
+    for (int i = 0; i < 2; ++i) {
+        const at::Tensor& s = tensor(PyTuple_GET_ITEM(cache, 2 + i));
+        on_device(h, s, "the cache's scales must be on the context's device");
+        require(s.scalar_type() == at::kFloat && s.is_contiguous() && s.dim() == 3 && s.size(0) == c.B && s.size(1) == c.H &&
+                    s.size(2) == nb, "the cache's scales are contiguous float32 [batch, heads, blocks of tokens]");
+        (i ? c.v_scale : c.k_scale) = static_cast<float*>(s.data_ptr());
+    }
+    if (given(PyTuple_GET_ITEM(cache, 4))) {
+        const at::Tensor& b = tensor(PyTuple_GET_ITEM(cache, 4));
+        on_device(h, b, "the cache's bounds must be on the context's device");
+        require(b.scalar_type() == at::kChar && b.is_contiguous() && b.dim() == 5 && b.size(0) == c.B && b.size(1) == c.H &&
+                    b.size(2) == nb && b.size(3) == 2 && b.size(4) == c.D,
+                "the cache's bounds are contiguous int8 [batch, heads, blocks of tokens, 2, head_dim]");
+        c.bounds = static_cast<int8_t*>(b.data_ptr());
+    }
+}
+
+const int32_t* per_sequence(const Host* h, const ltca_kv8_cache& c, PyObject* o, const char* msg) {
+    if (!given(o)) return nullptr;
+    const at::Tensor& n = tensor(o);
+    on_device(h, n, msg);
+    require(n.scalar_type() == at::kInt && n.is_contiguous() && n.dim() == 1 && n.size(0) == c.B, msg);
+    return static_cast<const int32_t*>(n.data_ptr());
+}
+constexpr const char* kKvLen = "kv_len must be contiguous int32 [batch] on the context's device";
+constexpr const char* kNewLen = "new_len must be contiguous int32 [batch] on the context's device";
+
+// (cache, k, v, kv_len, new_len)
+PyObject* kv8_append(Host* h, PyObject* const* a) {
+    ltca_kv8_cache c;
+    fill_cache(h, c, a[0]);
+    ltca_kv8_append_params p;
+    std::memset(&p, 0, sizeof(p));
+    const at::Tensor& k = tensor(a[1]);
+    const at::Tensor& v = tensor(a[2]);
+    on_device(h, k, "k and v must be on the context's device");
+    on_device(h, v, "k and v must be on the context's device");
+    require(k.dim() == 4 && k.size(2) <= INT32_MAX, "k must be [batch, heads, tokens, head_dim]");
+    same_shape(k, c.B, c.H, k.size(2), c.D, "k must be [batch, heads, tokens, head_dim] of the cache");
+    same_shape(v, c.B, c.H, k.size(2), c.D, "v must have the shape of k");
+    require(k.scalar_type() == v.scalar_type(), "k and v must have one dtype");
+    p.n = (int32_t)k.size(2);
+    p.dtype = float_type(k.scalar_type());
+    p.k = k.data_ptr(); p.k_strides = strides(k);
+    p.v = v.data_ptr(); p.v_strides = strides(v);
+    require(given(a[3]), kKvLen);
+    p.kv_len = per_sequence(h, c, a[3], kKvLen);
+    p.new_len = per_sequence(h, c, a[4], kNewLen);
+    check(h, unlocked([&] { return ltca_kv8_append(h->ctx, &c, &p); }));
+    Py_RETURN_NONE;
+}
+
+// (cache, kv_len, start, count or None, dtype or None, out_k, out_v): k, v
+PyObject* kv8_read(Host* h, PyObject* const* a) {
+    ltca_kv8_cache c;
+    fill_cache(h, c, a[0]);
+    ltca_kv8_read_params p;
+    std::memset(&p, 0, sizeof(p));
+    p.kv_len = per_sequence(h, c, a[1], kKvLen);
+    p.start = int32_of(a[2], "bad start");
+    const int64_t n = given(a[3]) ? integer(a[3]) : (int64_t)c.S - p.start;
+    require(p.start >= 0 && n >= 0 && p.start + n <= c.S, "start .. start + count must lie in the cache");
+    p.n = (int32_t)n;
+    at::ScalarType t = at::kBFloat16;
+    if (given(a[4])) {
+        if (!THPDtype_Check(a[4])) raise(PyExc_TypeError, "expected a dtype");
+        t = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    } else if (given(a[5])) {
+        t = tensor(a[5]).scalar_type();
+    }
+    p.dtype = float_type(t);
+    at::Tensor o[2];
+    for (int i = 0; i < 2; ++i) {
+        o[i] = given(a[5 + i]) ? tensor(a[5 + i]) : empty(h, {c.B, c.H, n, c.D}, t);
+        on_device(h, o[i], "out_k and out_v must be on the context's device");
+        same_shape(o[i], c.B, c.H, n, c.D, "out_k and out_v are [batch, heads, count, head_dim]");
+        require(o[i].scalar_type() == t, "out_k and out_v must have the dtype that is asked for");
+    }
+    p.k = o[0].data_ptr(); p.k_strides = strides(o[0]);
+    p.v = o[1].data_ptr(); p.v_strides = strides(o[1]);
+    check(h, unlocked([&] { return ltca_kv8_read(h->ctx, &c, &p); }));
+    return Py_BuildValue("NN", result(a[5], o[0]), result(a[6], o[1]));
+}
+
+template <typename Params>
+void fill_queries(const Host* h, const ltca_kv8_cache& c, Params& p, const at::Tensor& q) {
+    std::memset(&p, 0, sizeof(p));
+    on_device(h, q, "q must be on the context's device");
+    require(q.dim() == 4 && q.size(0) == c.B && q.size(3) == c.D && q.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX,
+            "q must be [batch, heads, queries, head_dim] of the cache");
+    p.Hq = (int32_t)q.size(1); p.Sq = (int32_t)q.size(2);
+    p.dtype = float_type(q.scalar_type());
+    p.q = q.data_ptr(); p.q_strides = strides(q);
+}
+
+// (q, cache, kv_len, new_len, scale, causal, keep_mask, score_clamp, blocks, out, lse): out, lse
+PyObject* kv8_decode(Host* h, PyObject* const* a) {
+    ltca_kv8_cache c;
+    fill_cache(h, c, a[1]);
+    ltca_kv8_decode_params p;
+    const at::Tensor& q = tensor(a[0]);
+    fill_queries(h, c, p, q);
+    p.kv_len = per_sequence(h, c, a[2], kKvLen);
+    p.new_len = per_sequence(h, c, a[3], kNewLen);
+    p.scale = given(a[4]) ? (float)number(a[4]) : (float)(1.0 / std::sqrt((double)c.D));
+    p.causal = truth(a[5]);
+    if (given(a[6])) {
+        const at::Tensor& m = tensor(a[6]);
+        on_device(h, m, "keep_mask must be on the context's device");
+        require(m.scalar_type() == at::kFloat && m.is_contiguous() && m.dim() == 3 && m.size(0) == c.B && m.size(1) == p.Sq &&
+                    m.size(2) == c.S, "keep_mask must be contiguous float32 [batch, queries, capacity]");
+        p.keep_mask = static_cast<const float*>(m.data_ptr());
+    }
+    p.score_clamp = given(a[7]) ? (float)number(a[7]) : 0.f;
+    if (given(a[8])) {
+        const at::Tensor& b = tensor(a[8]);
+        on_device(h, b, "blocks must be on the context's device");
+        require(b.scalar_type() == at::kInt && b.is_contiguous() && b.dim() == 3 && b.size(0) == c.B && b.size(1) == c.H &&
+                    b.size(2) <= INT32_MAX, "blocks must be contiguous int32 [batch, heads of keys, count]");
+        p.n_blocks = (int32_t)b.size(2);
+        require(p.n_blocks >= 1, "an empty list of blocks");
+        p.blocks = static_cast<const int32_t*>(b.data_ptr());
+    }
+    at::Tensor o = given(a[9]) ? tensor(a[9]) : empty(h, {c.B, p.Hq, p.Sq, c.D}, q.scalar_type());
+    at::Tensor lse = given(a[10]) ? tensor(a[10]) : empty(h, {c.B, p.Hq, p.Sq}, at::kFloat);
+    on_device(h, o, "out must be on the context's device");
+    on_device(h, lse, "lse must be on the context's device");
+    same_shape(o, c.B, p.Hq, p.Sq, c.D, "out must have the shape of q");
+    require(o.scalar_type() == q.scalar_type(), "out must have the dtype of q");
+    require(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 3 && lse.size(0) == c.B && lse.size(1) == p.Hq &&
+                lse.size(2) == p.Sq, "lse must be contiguous float32 [batch, heads, queries]");
+    p.o = o.data_ptr(); p.o_strides = strides(o);
+    p.lse = static_cast<float*>(lse.data_ptr());
+    size_t need = 0;
+    ltca_kv8_decode_workspace_bytes(&c, &p, &need);
+    // A block of its own for each call, and not the context's scratch: what a captured call was given stays with its graph.
+    at::Tensor ws;
+    if (need) {
+        ws = empty(h, {(int64_t)need}, at::kByte);
+        const auto mine = c10::cuda::getStreamFromExternal(h->stream, (c10::DeviceIndex)h->device);
+        if (mine.stream() != c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)h->device).stream())
+            c10::cuda::CUDACachingAllocator::recordStream(ws.storage().data_ptr(), mine);
+        p.workspace = ws.data_ptr();
+        p.workspace_bytes = need;
+    }
+    check(h, unlocked([&] { return ltca_kv8_decode(h->ctx, &c, &p); }));
+    return Py_BuildValue("NN", result(a[9], o), result(a[10], lse));
+}
+
+// (q, cache, kv_len, count, new_len, first, last, out): blocks
+PyObject* kv8_select(Host* h, PyObject* const* a) {
+    ltca_kv8_cache c;
+    fill_cache(h, c, a[1]);
+    ltca_kv8_select_params p;
+    fill_queries(h, c, p, tensor(a[0]));
+    p.kv_len = per_sequence(h, c, a[2], kKvLen);
+    p.count = int32_of(a[3], "bad count");
+    p.new_len = per_sequence(h, c, a[4], kNewLen);
+    p.first = int32_of(a[5], "bad first");
+    p.last = int32_of(a[6], "bad last");
+    require(p.count >= 1, "count must be positive");
+    at::Tensor o = given(a[7]) ? tensor(a[7]) : empty(h, {c.B, c.H, p.count}, at::kInt);
+    on_device(h, o, "out must be on the context's device");
+    require(o.scalar_type() == at::kInt && o.is_contiguous() && o.dim() == 3 && o.size(0) == c.B && o.size(1) == c.H &&
+                o.size(2) == p.count, "out must be contiguous int32 [batch, heads of keys, count]");
+    p.blocks = static_cast<int32_t*>(o.data_ptr());
+    check(h, unlocked([&] { return ltca_kv8_select(h->ctx, &c, &p); }));
+    return result(a[7], o);
+}
+
 // ---- the modules -------------------------------------------------------------------------------
 // x, wq, wk, wv, wo, B, S, H, head_width, scale, causal, time_major, use_residual, use_layer_norm, gamma, beta,
 // keep_mask, mode, bq, bk, bv, bo   (the first kModuleArgs arguments of every module call)
@@ -431,6 +639,13 @@ PyObject* host_workspace(Host* h, PyObject* const* a) {
     return wrap(std::move(ws));
 }
 
+// (address of the stream): the stream that the context's calls enqueue on from now on.
+PyObject* host_set_stream(Host* h, PyObject* const* a) {
+    h->stream = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(word64(a[0])));
+    ltca_ctx_set_stream(h->ctx, h->stream);
+    Py_RETURN_NONE;
+}
+
 // (): the context is gone; later calls fail with LTCA_ERR_INVALID.
 PyObject* host_close(Host* h, PyObject* const*) {
     h->ctx = nullptr;
@@ -464,21 +679,27 @@ PyMethodDef host_methods[] = {
     LTCA_METHOD(attn_fwd, 11),
     LTCA_METHOD(attn_bwd, 16),
     LTCA_METHOD(attn_decode, 9),
+    LTCA_METHOD(kv8_append, 5),
+    LTCA_METHOD(kv8_read, 7),
+    LTCA_METHOD(kv8_decode, 11),
+    LTCA_METHOD(kv8_select, 8),
     LTCA_METHOD(tsa_fwd, kModuleArgs + 2),
     LTCA_METHOD(tsa_bwd, kModuleArgs + 4),
     LTCA_METHOD(fa_fwd, kModuleArgs + 3),
     LTCA_METHOD(fa_bwd, kModuleArgs + 4),
     {"workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<host_workspace, 1>)), METH_FASTCALL, nullptr},
+    {"set_stream", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<host_set_stream, 1>)), METH_FASTCALL, nullptr},
     {"close", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<host_close, 0>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 int host_init(PyObject* self, PyObject* args, PyObject*) {
-    unsigned long long ctx = 0;
+    unsigned long long ctx = 0, stream = 0;
     int device = 0;
-    if (!PyArg_ParseTuple(args, "Ki", &ctx, &device)) return -1;
+    if (!PyArg_ParseTuple(args, "KiK", &ctx, &device, &stream)) return -1;
     Host* h = reinterpret_cast<Host*>(self);
     h->ctx = reinterpret_cast<ltca_ctx*>(static_cast<uintptr_t>(ctx));
     h->device = device;
+    h->stream = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
     if (!h->ws) h->ws = new at::Tensor();
     return 0;
 }
@@ -508,7 +729,7 @@ PyMODINIT_FUNC PyInit__host(void) {
     HostType.tp_name = "cuda_ltc_b200._host.Host";
     HostType.tp_basicsize = sizeof(Host);
     HostType.tp_flags = Py_TPFLAGS_DEFAULT;
-    HostType.tp_doc = "Calls of one ltca_ctx: Host(context address, device).";
+    HostType.tp_doc = "Calls of one ltca_ctx: Host(context address, device, stream address).";
     HostType.tp_new = PyType_GenericNew;
     HostType.tp_init = host_init;
     HostType.tp_dealloc = host_dealloc;

@@ -223,6 +223,110 @@ int ltca_attn_decode_workspace_bytes(const ltca_attn_params* p, size_t* bytes_ou
  */
 int ltca_attn_decode_static(void* stream, const ltca_attn_params* p, char* err, size_t err_len);
 
+/* ---- 8-bit key/value cache ----------------------------------------------------------------- */
+
+/*
+ * Keys and values of sequences that grow, in e4m3 (one sign, four exponent, three mantissa bits) with one scale for every
+ * block of tokens and head:  value = code * scale.  (No counterpart in the reference, which keeps no cache.)
+ *
+ * A scale is a power of two, the smallest from 2^-100 on by which the largest finite magnitude of its block comes down to
+ * e4m3's 448.  e4m3 has its own exponent, so that a finer scale would not make a value more exact, and with a power of two
+ * the division, a later change of the scale and the reading back round nothing that e4m3 itself does not.
+ *
+ * What lies behind a sequence's live length is never read: a cache and its scales need no clearing, neither when they are
+ * allocated nor when another sequence takes the place over.
+ */
+typedef struct {
+    int32_t  B, H;              /* sequences, heads of keys and values                                       */
+    int32_t  S, D;              /* capacity in tokens, any; head width, 32, 64 or 128                        */
+    int32_t  block;             /* tokens that share a scale: 16, 32, 64 or 128 (the last block may be short) */
+    void*    k; ltca_strides k_strides;        /* [B,H,S,D] e4m3, rows on 16-byte boundaries                 */
+    void*    v; ltca_strides v_strides;
+    float   *k_scale, *v_scale;                /* [B,H,ceil(S/block)] contiguous                             */
+    int8_t*  bounds;            /* [B,H,ceil(S/block),2,D] contiguous, 4-byte aligned: floor(min/4) and ceil(max/4) over the
+                                   codes of a block's live keys, for ltca_kv8_select; NULL: not kept              */
+} ltca_kv8_cache;
+
+/*
+ * Appends tokens.  kv_len counts a sequence's tokens WITH the new ones, as ltca_kv8_decode wants it, so that a step raises the
+ * lengths once and makes both calls with them: token i of sequence b goes to position kv_len[b] - new_len[b] + i.  Positions
+ * outside 0 .. S-1 are left out; tokens behind new_len[b] are not read.
+ * A block that the sequence had begun keeps its scale as long as the new tokens fit; where they do not it takes the larger one
+ * and its older codes are rounded again to it.  A block's first token sets its scale anew.  Infinities become +-448 times the
+ * scale, NaN stays NaN; neither counts for the scale (in the bounds NaN counts as both ends, -112 and 112).
+ */
+typedef struct {
+    int32_t n;                  /* tokens of k and v; 0: nothing is done             */
+    int32_t dtype;              /* ltca_dtype of k and v                             */
+    const void* k; ltca_strides k_strides;     /* [B,H,n,D], any alignment           */
+    const void* v; ltca_strides v_strides;
+    const int32_t* kv_len;      /* [B] length behind the call, not written           */
+    const int32_t* new_len;     /* optional [B] (0 .. n): new tokens of a sequence; NULL: n */
+} ltca_kv8_append_params;
+int ltca_kv8_append(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_append_params* p);
+
+/* Reads positions start .. start+n-1 back: k, v [B,H,n,D] = code * scale in fp32 or bf16 (exact in both, up to the type's own
+ * range); positions from kv_len[b] on give zeros.  What ltca_attn_fwd takes for the long chunk of a prompt. */
+typedef struct {
+    int32_t start, n;           /* 0 <= start, start + n <= S; n = 0: nothing is done */
+    int32_t dtype;              /* ltca_dtype of k and v                             */
+    void* k; ltca_strides k_strides;           /* [B,H,n,D], any alignment           */
+    void* v; ltca_strides v_strides;
+    const int32_t* kv_len;      /* optional [B]; NULL: all S                         */
+} ltca_kv8_read_params;
+int ltca_kv8_read(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_read_params* p);
+
+/*
+ * Attention of the newest tokens over the cache: O = softmax(mask(scale * Q K^T)) V.  Heads of queries may share a head of
+ * keys: head h reads head h / (Hq/H).  Query i of sequence b stands at position kv_len[b] - new_len[b] + i; rows from
+ * new_len[b] on, and rows that see no key, give zeros and lse = -inf.  Scores and statistics are fp32; products run on the
+ * tensor pipe with the codes as they are (e4m3 is exact in fp16) and Q and P in fp16, for fp32 queries in two fp16 terms each
+ * (22 bits).  A few tens of rows (new tokens x heads that share) per head of keys are what the kernel is made for; long
+ * chunks of a prompt are faster through ltca_kv8_read and ltca_attn_fwd.
+ */
+typedef struct {
+    int32_t Hq, Sq;             /* heads of queries (a multiple of H); newest tokens, one or more */
+    int32_t dtype;              /* ltca_dtype of q and o                             */
+    int32_t causal;             /* key j visible to a query at position t iff j <= t */
+    float   scale;              /* > 0                                               */
+    float   score_clamp;        /* > 0: s = min(s, score_clamp) after scaling        */
+    const void* q; ltca_strides q_strides;     /* [B,Hq,Sq,D], any alignment         */
+    void*       o; ltca_strides o_strides;     /* [B,Hq,Sq,D], any alignment         */
+    float*      lse;            /* optional [B,Hq,Sq]                                */
+    const float*   keep_mask;   /* optional [B,Sq,S] contiguous; value 0 hides the key */
+    const int32_t* kv_len;      /* optional [B], with the new tokens; NULL: all S    */
+    const int32_t* new_len;     /* optional [B] (0 .. Sq); NULL: Sq                  */
+    const int32_t* blocks;      /* optional [B,H,n_blocks]: only keys of these blocks of tokens are read.  Entries below 0 or
+                                   behind the last live block stand for none; a block that is listed twice counts twice */
+    int32_t n_blocks;
+    void*  workspace;           /* ltca_kv8_decode_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} ltca_kv8_decode_params;
+int ltca_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decode_params* p);
+/* Zero where no more than 16 CTAs work on a sequence's head of keys. */
+int ltca_kv8_decode_workspace_bytes(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p, size_t* bytes_out);
+
+/*
+ * Which `count` blocks of tokens of each sequence and head of keys the newest tokens should read.  Each row of Q (a new token
+ * and a head of queries) is rounded to eight bits with a power-of-two step, the smallest from 2^-100 on by which its largest
+ * finite magnitude comes down to 127; a block's score is the largest over the rows of
+ *     sum_d max(q_d lo_d, q_d hi_d) * k_scale * step       (lo, hi: the block's bounds)
+ * which no product of that row with one of the block's keys exceeds by more than the rounding of Q; the sum is one of whole
+ * numbers, so that the choice does not depend on an order of additions.  NaN in Q counts as zero, an infinity as +-127.  The `first` blocks and the `last` live ones are
+ * always taken; equal scores go to the lower index.  blocks: the indices in rising order, then -1 where a sequence has fewer.
+ */
+typedef struct {
+    int32_t Hq, Sq;
+    int32_t dtype;              /* ltca_dtype of q                                   */
+    const void* q; ltca_strides q_strides;     /* [B,Hq,Sq,D], any alignment         */
+    const int32_t* kv_len;      /* optional [B], with the new tokens; NULL: all S    */
+    const int32_t* new_len;     /* optional [B] (0 .. Sq): rows that count (none: all scores are equal); NULL: Sq */
+    int32_t first, last;        /* each >= 0, first + last <= count                  */
+    int32_t count;              /* >= 1                                              */
+    int32_t* blocks;            /* [B,H,count], written whole                        */
+} ltca_kv8_select_params;
+int ltca_kv8_select(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_select_params* p);
+
 /* ---- TimeSelfAttention module ----------------------------------------------------------- */
 
 /*
