@@ -238,7 +238,7 @@ int ltca_attn_decode_static(void* stream, const ltca_attn_params* p, char* err, 
  */
 typedef struct {
     int32_t  B, H;              /* sequences, heads of keys and values                                       */
-    int32_t  S, D;              /* capacity in tokens, any; head width, 32, 64 or 128                        */
+    int32_t  S, D;              /* capacity in tokens, up to 2^30; head width, 32, 64 or 128                 */
     int32_t  block;             /* tokens that share a scale: 16, 32, 64 or 128 (the last block may be short) */
     void*    k; ltca_strides k_strides;        /* [B,H,S,D] e4m3, rows on 16-byte boundaries                 */
     void*    v; ltca_strides v_strides;
