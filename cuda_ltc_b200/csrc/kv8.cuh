@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "sm100_ptx.cuh"
 
