@@ -36,7 +36,7 @@ int check_cache(ltca_ctx* ctx, const ltca_kv8_cache* c, bool k, bool v) {
         return fail(ctx, LTCA_ERR_INVALID, "null tensor in the cache");
     if ((k && misaligned(c->k, c->k_strides, 16)) || (v && misaligned(c->v, c->v_strides, 16)))
         return fail(ctx, LTCA_ERR_INVALID, "the cache's rows must start on 16-byte boundaries");
-    if (reinterpret_cast<uintptr_t>(c->bounds) % 4) return fail(ctx, LTCA_ERR_INVALID, "bounds must be 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(c->bounds) % 16) return fail(ctx, LTCA_ERR_INVALID, "bounds must be 16-byte aligned");
     return LTCA_OK;
 }
 int check_dtype(ltca_ctx* ctx, int dtype) {

@@ -1,4 +1,14 @@
 // Which blocks of an 8-bit cache the newest tokens should read: see ltca_kv8_select in include/ltc_attn.h.
+//
+// One cluster of CTAs takes a pair (sequence, head of keys), each CTA a run of its blocks; scores never leave shared memory.
+//   - Scores: Q in eight bits and the bounds are whole numbers, so that four channels cost a byte mask (the sign of q picks the
+//     lower or the upper bound), a selection and a four-way dot product.  The sum is below 2^21 and exact.
+//   - The `count` best: the score's bits in an order that whole numbers have, and a search for the count-th largest of them
+//     eight bits at a time: histograms in shared memory, added over the cluster.  Two to four rounds.
+//   - The indices come out in rising order, since every CTA knows how many the ones before it have taken.
+// Bound by memory for long caches (2 D + 4 bytes a block), by the barriers of the search for short ones.
+#include <cooperative_groups.h>
+
 #include "kv8.cuh"
 
 namespace ltca {
@@ -8,7 +18,9 @@ namespace {
 struct SelectArgs {
     ltca_kv8_cache c;
     ltca_kv8_select_params p;
-    int nb, rows;
+    int nb, G, R;               // blocks of tokens; heads of queries per head of keys; rows of a pair
+    int ctas;                   // of a pair, one cluster
+    int room;                   // scores that a CTA has room for
 };
 
 // Numbers in the order of the scores; 0 is below every score's, the largest above.
@@ -17,84 +29,245 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kThreads = 256;
+// 0xff for each byte below zero (a selector's highest bit replicates the byte's sign).
+__device__ __forceinline__ uint32_t signs(uint32_t x) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %1, 0xba98;" : "=r"(r) : "r"(x));
+    return r;
+}
 
-// One CTA per sequence and head of keys; the scores' order stays in shared memory, and a block's rank is counted.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) kv8_select_kernel(const SelectArgs a) {
+constexpr int kThreads = 256, kSelectWarps = kThreads / 32;
+constexpr int kRowsAtATime = 32;            // rows of Q in shared memory
+constexpr int kMaxSelectCluster = 16;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) kv8_select_kernel(const __grid_constant__ SelectArgs a) {
+    constexpr int kLanes = D / 16;                                  // of a block: each has 16 channels of both bounds
+    constexpr int kPerWarp = 32 / kLanes;
     extern __shared__ __align__(16) unsigned char smem[];
-    uint32_t* key = reinterpret_cast<uint32_t*>(smem);
-    __shared__ int8_t qi[128];
-    __shared__ uint32_t sm_max;
-    __shared__ int sm_base[kThreads / 32 + 1];
+    uint32_t* key = reinterpret_cast<uint32_t*>(smem);              // [room]
+    __shared__ __align__(16) int8_t sm_q[kRowsAtATime][D];
+    __shared__ float sm_step[kRowsAtATime];
+    __shared__ uint32_t sm_hist[4][256];
+    __shared__ uint32_t sm_warp[2][kSelectWarps];
+    __shared__ uint32_t sm_digit, sm_above, sm_here;
+    __shared__ uint32_t sm_count[2];                                // of this CTA's scores: above the threshold, at it
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
     grid_dependency_wait();
-    const int b = blockIdx.x / a.c.H, h = blockIdx.x % a.c.H, D = a.c.D, G = a.p.Hq / a.c.H, tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = (int)(blockIdx.x % a.ctas);
+    const int64_t pair = blockIdx.x / a.ctas;
+    const int b = (int)(pair / a.c.H), h = (int)(pair % a.c.H);
     const int live = a.p.kv_len ? min(max(a.p.kv_len[b], 0), a.c.S) : a.c.S;
     const int blocks = (live + a.c.block - 1) / a.c.block;
-    const int n = new_tokens(a.p.new_len, b, a.p.Sq);
-    const int64_t pair = (int64_t)b * a.c.H + h;
-    const int8_t* bounds = a.c.bounds + pair * a.nb * 2 * D;
-    const float* scale = a.c.k_scale + pair * a.nb;
+    const int n = new_tokens(a.p.new_len, b, a.p.Sq), rows = a.G * n;
     int32_t* out = a.p.blocks + pair * a.p.count;
-    for (int j = tid; j < blocks; j += kThreads) key[j] = order_of(-INFINITY);
-    for (int r = 0; r < G * n; ++r) {
-        const T* q = reinterpret_cast<const T*>(a.p.q) + b * a.p.q_strides.batch + (h * G + r / n) * a.p.q_strides.head +
-                     (r % n) * a.p.q_strides.seq;
-        if (tid == 0) sm_max = 0;
-        __syncthreads();
-        if (tid < D) atomicMax(&sm_max, finite_abs_bits(ld_value(q + tid)));
-        __syncthreads();
-        const float step = pow2(int8_exponent(sm_max));
-        if (tid < D) {
-            const float x = ld_value(q + tid) / step;
-            qi[tid] = x == x ? (int8_t)rintf(fminf(fmaxf(x, -127.f), 127.f)) : (int8_t)0;
-        }
-        __syncthreads();
-        for (int j = tid; j < blocks; j += kThreads) {
-            int sum = 0;
-            for (int d = 0; d < D; ++d) sum += max(qi[d] * bounds[j * 2 * D + d], qi[d] * bounds[j * 2 * D + D + d]);
-            const float s = (float)sum * scale[j] * step;
-            if (s == s) key[j] = max(key[j], order_of(s));
-        }
-        __syncthreads();
+    const int per = (blocks + a.ctas - 1) / a.ctas;                 // <= room
+    const int j0 = min(rank * per, blocks), mine = min(per, blocks - j0);
+
+    const int total = min(a.p.count, blocks);
+    for (int i = total + rank * kThreads + tid; i < a.p.count; i += a.ctas * kThreads) out[i] = -1;
+    if (blocks <= a.p.count) {                                      // all of them, in every CTA of the cluster alike
+        for (int i = rank * kThreads + tid; i < blocks; i += a.ctas * kThreads) out[i] = i;
+        return;
     }
-    for (int j = tid; j < blocks; j += kThreads)
-        if (j < a.p.first || j >= blocks - a.p.last) key[j] = 0xffffffffu;
+    for (int i = tid; i < 4 * 256; i += kThreads) (&sm_hist[0][0])[i] = 0;
+    if (tid < 2) sm_count[tid] = 0;
+
+    // ---- scores ----
+    const uint32_t floor_key = order_of(-INFINITY);
+    const int8_t* bounds = a.c.bounds + (pair * a.nb + j0) * 2 * D;
+    const float* scale = a.c.k_scale + pair * a.nb + j0;
+    const int sub = lane % kLanes, slot = lane / kLanes;
+    int r0 = 0;
+    do {
+        const int batch = min(rows - r0, kRowsAtATime);
+        if (r0) __syncthreads();
+        for (int r = warp; r < batch; r += kSelectWarps) {
+            const int i = (r0 + r) / a.G, g = (r0 + r) % a.G;
+            const T* q = reinterpret_cast<const T*>(a.p.q) + b * a.p.q_strides.batch + (int64_t)(h * a.G + g) * a.p.q_strides.head +
+                         (int64_t)i * a.p.q_strides.seq;
+            float x[D / 32];
+            uint32_t most = 0;
+#pragma unroll
+            for (int y = 0; y < D / 32; ++y) {
+                x[y] = ld_value(q + lane + 32 * y);
+                most = max(most, finite_abs_bits(x[y]));
+            }
+            const int e = int8_exponent(__reduce_max_sync(0xffffffffu, most));
+            const float down = pow2(-e);
+#pragma unroll
+            for (int y = 0; y < D / 32; ++y) {
+                const float v = x[y] * down;
+                sm_q[r][lane + 32 * y] = v == v ? (int8_t)rintf(fminf(fmaxf(v, -127.f), 127.f)) : (int8_t)0;
+            }
+            if (lane == 0) sm_step[r] = pow2(e);
+        }
+        __syncthreads();
+        for (int base = warp * kPerWarp; base < mine; base += kSelectWarps * kPerWarp) {
+            const int j = base + slot;
+            const bool there = j < mine;
+            uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+            float ks = 0.f;
+            if (there) {
+                const uint4* p = reinterpret_cast<const uint4*>(bounds + (int64_t)j * 2 * D) + sub;
+                lo = __ldg(p);
+                hi = __ldg(p + kLanes);
+                ks = __ldg(scale + j);
+            }
+            uint32_t best = r0 && there ? key[j] : floor_key;
+            for (int r = 0; r < batch; ++r) {
+                const uint4 q = *reinterpret_cast<const uint4*>(&sm_q[r][sub * 16]);
+                int sum = 0;
+                auto four = [&](uint32_t qw, uint32_t l, uint32_t u) {
+                    const uint32_t neg = signs(qw);
+                    sum = __dp4a((int)qw, (int)((l & neg) | (u & ~neg)), sum);
+                };
+                four(q.x, lo.x, hi.x); four(q.y, lo.y, hi.y); four(q.z, lo.z, hi.z); four(q.w, lo.w, hi.w);
+#pragma unroll
+                for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                const float s = (float)sum * ks * sm_step[r];
+                if (s == s) best = max(best, order_of(s));
+            }
+            if (there && sub == 0) {
+                const int at = j0 + j;
+                if (r0 + batch == rows && (at < a.p.first || at >= blocks - a.p.last)) best = 0xffffffffu;
+                key[j] = best;
+            }
+        }
+        r0 += batch;
+    } while (r0 < rows);
     __syncthreads();
-    int done = 0;
-    for (int j0 = 0; j0 < blocks; j0 += kThreads) {
-        const int j = j0 + tid;
-        bool take = false;
-        if (j < blocks) {
-            int rank = 0;
-            const uint32_t mine = key[j];
-            for (int i = 0; i < blocks; ++i) rank += key[i] > mine || (key[i] == mine && i < j);
-            take = rank < a.p.count;
+
+    // ---- the count-th largest ----
+    uint32_t prefix = 0, known = 0;                                 // its leading bits, and a mask of them
+    uint32_t need = (uint32_t)a.p.count;                            // how many of those that share them are wanted
+    uint32_t at_prefix = 0;                                         // and how many do
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        for (int i = tid; i < mine; i += kThreads) {
+            const uint32_t k = key[i];
+            if ((k & known) == prefix) atomicAdd(&sm_hist[pass][(k >> shift) & 255], 1u);
         }
-        const uint32_t vote = __ballot_sync(0xffffffffu, take);
-        if ((tid & 31) == 0) sm_base[tid >> 5] = __popc(vote);
+        cluster.sync();
+        uint32_t mysum = 0;
+        for (int k = 0; k < a.ctas; ++k) mysum += *cluster.map_shared_rank(&sm_hist[pass][tid], k);
+        // how many lie in digits above this thread's
+        uint32_t run = mysum;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t o = __shfl_down_sync(0xffffffffu, run, off);
+            if (lane + off < 32) run += o;
+        }
+        if (lane == 0) sm_warp[0][warp] = run;
         __syncthreads();
-        int at = done;
-        for (int w = 0; w < (tid >> 5); ++w) at += sm_base[w];
-        if (take) out[at + __popc(vote & ((1u << (tid & 31)) - 1))] = j;
-        for (int w = 0; w < kThreads / 32; ++w) done += sm_base[w];
+        uint32_t above = run - mysum;
+        for (int w = warp + 1; w < kSelectWarps; ++w) above += sm_warp[0][w];
+        if (above < need && above + mysum >= need) { sm_digit = (uint32_t)tid; sm_above = above; sm_here = mysum; }
+        __syncthreads();
+        prefix |= sm_digit << shift;
+        known |= 255u << shift;
+        need -= sm_above;
+        at_prefix = sm_here;
+        if (at_prefix == need) break;                               // all that share the prefix are wanted
         __syncthreads();
     }
-    for (int i = done + tid; i < a.p.count; i += kThreads) out[i] = -1;
+    // ---- the indices ----
+    // above: the known bits are larger; at: they are the prefix
+    uint32_t n_above = 0, n_at = 0;
+    for (int i = tid; i < mine; i += kThreads) {
+        const uint32_t k = key[i] & known;
+        n_above += k > prefix;
+        n_at += k == prefix;
+    }
+    n_above = __reduce_add_sync(0xffffffffu, n_above);
+    n_at = __reduce_add_sync(0xffffffffu, n_at);
+    if (lane == 0) {
+        atomicAdd(&sm_count[0], n_above);
+        atomicAdd(&sm_count[1], n_at);
+    }
+    cluster.sync();
+    uint32_t done = 0, left = need;                                 // places that are taken; how many at the threshold still may be
+    for (int k = 0; k < rank; ++k) {
+        const uint32_t x = *cluster.map_shared_rank(&sm_count[0], k), y = *cluster.map_shared_rank(&sm_count[1], k);
+        const uint32_t take = min(y, left);
+        done += x + take;
+        left -= take;
+    }
+    for (int base = 0; base < mine; base += kThreads) {
+        const int i = base + tid;
+        const uint32_t k = i < mine ? key[i] & known : 0u;
+        const bool up = i < mine && k > prefix, at = i < mine && k == prefix;
+        const uint32_t vote_up = __ballot_sync(0xffffffffu, up), vote_at = __ballot_sync(0xffffffffu, at), below = (1u << lane) - 1;
+        if (lane == 0) { sm_warp[0][warp] = __popc(vote_up); sm_warp[1][warp] = __popc(vote_at); }
+        __syncthreads();
+        uint32_t ups = 0, ats = 0, all_up = 0, all_at = 0;
+        for (int w = 0; w < kSelectWarps; ++w) {
+            if (w < warp) { ups += sm_warp[0][w]; ats += sm_warp[1][w]; }
+            all_up += sm_warp[0][w];
+            all_at += sm_warp[1][w];
+        }
+        ups += __popc(vote_up & below);
+        ats += __popc(vote_at & below);
+        if (up || (at && ats < left)) out[done + ups + min(ats, left)] = j0 + i;
+        const uint32_t take = min(all_at, left);
+        done += all_up + take;
+        left -= take;
+        __syncthreads();
+    }
+    cluster.sync();                                                 // until nobody reads this CTA's shared memory
+}
+
+template <typename T, int D>
+int launch(ltca_ctx* ctx, const SelectArgs& a) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)((int64_t)a.c.B * a.c.H * a.ctas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)a.room * 4;
+    cfg.stream = ctx->stream;
+    static SmemOptIn once;
+    if (cfg.dynamicSmemBytes > 32 * 1024)
+        LTCA_CUDA_OK(ctx, opt_in_dynamic_smem(once, ctx->device, kv8_select_kernel<T, D>, 200 * 1024));
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.ctas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.ctas > 1 ? 2 : 1;
+    if (a.ctas > 8) {
+        static SmemOptIn wide;      // clusters of more than eight CTAs are an opt-in of a kernel on one device
+        const uint64_t bit = (ctx->device >= 0 && ctx->device < 64) ? (1ull << ctx->device) : 0ull;
+        if (!bit || !(wide.done.load(std::memory_order_acquire) & bit)) {
+            LTCA_CUDA_OK(ctx, cudaFuncSetAttribute(kv8_select_kernel<T, D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            wide.done.fetch_or(bit, std::memory_order_release);
+        }
+    }
+    LTCA_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kv8_select_kernel<T, D>, a));
+    return LTCA_OK;
+}
+template <typename T>
+int launch_width(ltca_ctx* ctx, const SelectArgs& a) {
+    return a.c.D == 32 ? launch<T, 32>(ctx, a) : a.c.D == 64 ? launch<T, 64>(ctx, a) : launch<T, 128>(ctx, a);
 }
 
 }  // namespace
 
 int launch_kv8_select(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_select_params* p) {
-    SelectArgs a{*c, *p, (c->S + c->block - 1) / c->block, p->Hq / c->H * p->Sq};
-    const int bytes = a.nb * 4;
-    if (bytes > 200 * 1024) return fail(ctx, LTCA_ERR_UNSUPPORTED, "select: %d blocks of tokens are too many", a.nb);
-    auto kern = p->dtype == LTCA_BF16 ? kv8_select_kernel<__nv_bfloat16> : kv8_select_kernel<float>;
-    static SmemOptIn once[2];
-    LTCA_CUDA_OK(ctx, opt_in_dynamic_smem(once[p->dtype == LTCA_BF16], ctx->device, kern, 200 * 1024));
-    const dim3 grid((unsigned)(c->B * c->H));
-    LTCA_CUDA_OK(ctx, launch_dependent(kern, grid, dim3(kThreads), bytes, ctx->stream, a));
-    return LTCA_OK;
+    SelectArgs a{*c, *p, (c->S + c->block - 1) / c->block, p->Hq / c->H, p->Hq / c->H * p->Sq, 1, 0};
+    // about two CTAs per SM, each with 64 blocks at least
+    const int64_t pairs = (int64_t)c->B * c->H;
+    while (a.ctas < kMaxSelectCluster && pairs * a.ctas < 2 * kPlanSms && a.nb / (2 * a.ctas) >= 64) a.ctas *= 2;
+    while (a.ctas < kMaxSelectCluster && (a.nb + a.ctas - 1) / a.ctas > 48 * 1024) a.ctas *= 2;
+    a.room = (a.nb + a.ctas - 1) / a.ctas;
+    if (a.room > 48 * 1024) return fail(ctx, LTCA_ERR_UNSUPPORTED, "select: %d blocks of tokens are too many", a.nb);
+    if (pairs * a.ctas > 0x7fffffff) return fail(ctx, LTCA_ERR_INVALID, "select: too many sequences and heads for one call");
+    return p->dtype == LTCA_BF16 ? launch_width<__nv_bfloat16>(ctx, a) : launch_width<float>(ctx, a);
 }
 
 }  // namespace ltca

@@ -243,7 +243,7 @@ typedef struct {
     void*    k; ltca_strides k_strides;        /* [B,H,S,D] e4m3, rows on 16-byte boundaries                 */
     void*    v; ltca_strides v_strides;
     float   *k_scale, *v_scale;                /* [B,H,ceil(S/block)] contiguous                             */
-    int8_t*  bounds;            /* [B,H,ceil(S/block),2,D] contiguous, 4-byte aligned: floor(min/4) and ceil(max/4) over the
+    int8_t*  bounds;            /* [B,H,ceil(S/block),2,D] contiguous, 16-byte aligned: floor(min/4) and ceil(max/4) over the
                                    codes of a block's live keys, for ltca_kv8_select; NULL: not kept              */
 } ltca_kv8_cache;
 

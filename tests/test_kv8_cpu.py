@@ -72,7 +72,7 @@ def test_struct_layouts_match_the_header(tmp_path):
 BAD_CACHES = [
     (dict(B=0), -1, b"shape"), (dict(H=0), -1, b"shape"), (dict(S=0), -1, b"shape"), (dict(S=2 ** 30 + 1), -2, b"capacity"), (dict(D=48), -2, b"head_dim"),
     (dict(D=256), -2, b"head_dim"), (dict(block=8), -2, b"tokens"), (dict(block=48), -2, b"tokens"),
-    (dict(bounds=66), -1, b"bounds"), (dict(B=1 << 20, H=1 << 12), -1, b"B * H"),
+    (dict(bounds=72), -1, b"bounds"), (dict(B=1 << 20, H=1 << 12), -1, b"B * H"),
 ]
 BAD_CALLS = [
     ("ltca_kv8_append", dict(n=-1), {}, -1, b"negative"), ("ltca_kv8_append", dict(dtype=2), {}, -1, b"dtype"),
