@@ -10,39 +10,78 @@
 // which keeps bf16's 8 bits; fp32 rows travel in two fp16 terms (22 bits), and so do their weights.
 //
 // The order of the contracted index is free as long as both operands agree.  A lane therefore takes whole pieces of rows: of
-// K, 4 D/16 consecutive-by-16 bytes of two keys; of V, D/8 bytes of four keys, whose bytes a permutation brings side by side.
-// What a lane fetches (cp.async into slots of its own) is what it multiplies: the ring needs no barrier but the wait.
+// K, D/4 bytes of two keys; of V, D/8 bytes of four keys, whose bytes a permutation brings side by side.  The rows come by TMA
+// into a ring of the warp's own (a lane issues a step's copies; full bandwidth wants some 130 KB on their way to an SM, and with
+// cp.async the warps stood in line to issue them).
 //
 // Softmax.  With t the score in powers of two, a row keeps a reference m and e (whole numbers) and
 //     l = sum 2^(t - m),      O = sum 2^(t - m) (v_scale 2^(6 - e)) code.
 // e makes room for values of any size in fp16's range: weights lie around 2^6 where they matter, are as fine as 2^-24, and may
 // rise to 2^14 before m and e have to move.  So the usual step asks one vote of the warp instead of a reduction of maxima and
 // a multiplication of O, and every factor that ever touches O is a power of two.
-#include <cooperative_groups.h>
-
+//
+// Every warp works for itself.  The steps of all units (a pair and up to 8 NT of its rows) lie in one line, each unit's behind
+// a blank that stands for what a unit costs beside them, and a warp takes an equal run of it, whatever the lengths; it fetches
+// across the borders of units, so that the stream does not stop while a unit's queries are brought in or its sums leave.  A unit that one warp has seen whole is finished by it; shares
+// of a unit go to scratch and are joined by a second kernel.
 #include "kv8.cuh"
 
 namespace ltca {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;                   // of a CTA
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;                  // steps of a warp's keys in shared memory, all but one of them in flight
-constexpr int kMaxCluster = 16;             // CTAs of one pair that merge through shared memory
-constexpr int kStepBytes = 4096;            // keys and values of a warp's step: KG groups of 16 keys
-constexpr int kHead = 64;                   // a step's scales and positions
+constexpr int kHead = 48;                   // a step's positions and scales
+constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do
+constexpr int kUnitCost = 2;                // what a unit costs beside its steps, in steps
+constexpr int kNowhere = 0x7fffffff;        // the position of a group that is not there
 constexpr float kNone = -3.402823466e38f;   // the reference of a row that has seen no key
 constexpr float kLimit = 16384.f;           // largest weight before the references move
+
+// A warp's ring: its steps are SG groups of 16 keys, 4 to 8 KB, and all but one are in flight.
+constexpr int step_groups(int D) { return D == 32 ? 4 : 2; }
+template <int D> constexpr int kGroups = step_groups(D);
+template <int D> constexpr int kStepBytes = kGroups<D> * 32 * D;
+template <int D> constexpr int kStages = D == 128 ? 2 : 4;
+// CTAs of an SM, by the registers that NT tiles of 8 rows take
+constexpr int ctas_per_sm(int D, int nt) { return nt == 4 || nt * D >= 256 ? 2 : 3; }
+template <int D, int NT> constexpr int kCtas = ctas_per_sm(D, NT);
+// Tiles of 8 rows that a warp keeps at most: fp32's two terms of 128 channels leave room for two.
+constexpr int most_tiles(int es, int D) { return es == 4 && D == 128 ? 2 : 4; }
 
 struct DecodeArgs {
     ltca_kv8_cache c;
     ltca_kv8_decode_params p;
     int nb, G, R;               // blocks of tokens; heads of queries per head of keys; rows of a pair
-    int tiles;                  // of 8 NT rows
-    int nsplit, cluster;        // CTAs of a tile; whether they are a cluster
-    float* partial;             // [pairs * tiles][nsplit][8 NT][D + 3] where they are not
+    int tiles, rows;            // of a pair: tiles of 8 NT rows; rows of a tile that exist (of the first one)
+    int warps;                  // that share the line of steps
+    int vec_q, vec_o;           // rows of q start on boundaries of four values, rows of o on 16 bytes
+    int mask_rows;              // rows of keep_mask that a tile's rows need
+    int box;                    // keys of a copy
+    int strides;                // what has a stride of its own: sequences of k (1) and v (4), heads of k (2) and v (8)
+    float* partial;             // [2 warps][rows][D + 4]
+    uint32_t* status;
 };
+
+// Steps of each unit of sequence b.
+__device__ __forceinline__ int steps_of(const DecodeArgs& a, int b) {
+    const int len = a.p.kv_len ? a.p.kv_len[b] : a.c.S, live = min(max(len, 0), a.c.S);
+    if (live == 0) return 0;
+    const int sg = step_groups(a.c.D);
+    if (a.p.blocks) return (a.p.n_blocks * (a.c.block >> 4) + sg - 1) / sg;
+    return (live + 16 * sg - 1) / (16 * sg);
+}
+__device__ __forceinline__ int64_t cost_of(const DecodeArgs& a, int b) {                     // of all its units
+    const int steps = steps_of(a, b);
+    return steps == 0 ? 0 : (int64_t)(steps + kUnitCost) * (a.c.H * a.tiles);
+}
+// Warps that get a run of the line; where warp w's begins; whose a place is.
+__device__ __forceinline__ int warps_of(const DecodeArgs& a, int64_t total) {
+    return (int)min((int64_t)a.warps, (total + kMinCost - 1) / kMinCost);
+}
+__device__ __forceinline__ int64_t run_begin(int64_t total, int warps, int w) { return total * w / warps; }
+__device__ __forceinline__ int warp_of(int64_t total, int warps, int64_t at) { return (int)(((at + 1) * warps - 1) / total); }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -64,265 +103,431 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ void codes_to_half2(uint32_t four, uint32_t& low, uint32_t& high) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(low), "=r"(high) : "r"(four));
+}
 template <int N>
 __device__ __forceinline__ void fetch(uint32_t dst, const void* src) {
     if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
-
-// How a warp's step of KG groups of 16 keys lies in its ring, for a lane (r, c) = (lane / 4, lane % 4).
-template <int D>
-struct Step {
-    static constexpr int KG = 128 / D;
-    static constexpr int kParts = D == 128 ? 2 : 1;               // pieces of a key's row of K
-    static constexpr int kPart = D == 32 ? 8 : 16;                // their bytes
-    static constexpr int kVPart = D / 8;                          // bytes of a key's row of V
-    static constexpr int kWords = D / 16;                         // words of K per key and lane: one per product
-    static constexpr int kGroupLane = 2 * D / 16 * 8;             // bytes of a group per lane: D / 2 of K, D / 2 of V
-    // K: bytes of the row that words 4 part .. hold
-    static __device__ __forceinline__ int k_offset(int c, int part) { return part * 64 + c * kPart; }
-    static __device__ __forceinline__ int k_dim(int c, int word) {
-        return D == 32 ? c * 8 + 4 * word : (word >> 2) * 64 + c * 16 + 4 * (word & 3);
+__device__ __forceinline__ void load4(const float* p, bool vec, float (&x)[4]) {
+    if (vec) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(p));
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = p[i];
     }
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, bool vec, float (&x)[4]) {
+    if (vec) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+        x[0] = __uint_as_float(u.x << 16); x[1] = __uint_as_float(u.x & 0xffff0000u);
+        x[2] = __uint_as_float(u.y << 16); x[3] = __uint_as_float(u.y & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+    }
+}
+__device__ __forceinline__ void store4(float* p, bool vec, const float (&x)[4]) {
+    if (vec) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = x[i];
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, bool vec, const float (&x)[4]) {
+    if (vec) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(x[i]);
+    }
+}
+
+// How a group of 16 keys lies in the ring, rows of D bytes as TMA leaves them (128-byte swizzle for D = 128, 64-byte for 64), and
+// which pieces a lane (r, c) = (lane / 4, lane % 4) takes: of K's rows r and r + 8 the 16-byte chunks c and c + 4 (D = 32: 8
+// bytes), of V's rows 2c, 2c + 1, 2c + 8, 2c + 9 the D/8 bytes at r D/8.  Rows eight apart lie alike.
+template <int D>
+struct Group {
+    static constexpr int kParts = D == 128 ? 2 : 1;               // pieces of a key's row of K
+    static constexpr int kWords = D == 32 ? 2 : 4;                // words of a piece
+    static constexpr int kBytes = 16 * D;                         // of K, or of V
+    static __device__ __forceinline__ int swizzled(int row, int byte) {
+        if (D == 128) return row * 128 + (byte ^ (row & 7) << 4);
+        if (D == 64) return row * 64 + (byte ^ (row >> 1 & 3) << 4);
+        return row * 32 + byte;
+    }
+    // channel of word w of a lane's bytes of K
+    static __device__ __forceinline__ int k_dim(int c, int w) { return D == 32 ? c * 8 + 4 * w : (w >> 2) * 64 + c * 16 + 4 * (w & 3); }
 };
 
-// m, e, l of rows merge like this, and their O with the factor that comes back (o = O * 2^(E - 6) / L at the end).
-struct Merged { float M, E, L; };
-
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv8_decode_kernel(const __grid_constant__ DecodeArgs a) {
-    using St = Step<D>;
-    constexpr int KG = St::KG, MTD = D / 16, ROWS = 8 * NT;
+__global__ void __launch_bounds__(kThreads, kCtas<D, NT>)
+kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using Gr = Group<D>;
+    constexpr int W = D / 16, ROWS = 8 * NT;                      // products of a score; also tiles of 16 channels of O
     constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
     constexpr bool kQRegs = NT * kTerms * D <= 256;               // Q's fragments stay in registers
+    constexpr int ST = kStages<D>, SG = kGroups<D>;
+    constexpr int NG = NT == 4 ? 1 : 2;                           // groups whose products interleave, as the registers allow
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ __align__(16) uint2 sm_q[NT][kTerms][MTD][32];     // Q's fragments: b0, b1 of each product
-    __shared__ float sm_c[ROWS];                                  // what a row's S is multiplied by (times the key's scale)
-    __shared__ int sm_lim[ROWS], sm_i[ROWS];                      // keys below it are seen; which of the new tokens
-    __shared__ float sm_m[kWarps][ROWS], sm_e[kWarps][ROWS], sm_l[kWarps][ROWS];
-    __shared__ Merged sm_row[ROWS];
-    namespace cg = cooperative_groups;
+    __shared__ __align__(16) uint2 sm_q[kQRegs ? 1 : kWarps][kQRegs ? 1 : NT][kQRegs ? 1 : kTerms][kQRegs ? 1 : W][32];
+    __shared__ __align__(8) uint64_t sm_bar[kWarps][ST];
+    __shared__ int64_t sm_before[kThreads + 1];                   // the line up to each thread's sequences
+    __shared__ int64_t sm_warp[kWarps];
+    __shared__ uint32_t sm_abort;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
+    if (lane < ST) mbar_init(smem_u32(&sm_bar[warp][lane]), 1);
+    mbar_fence_init();
+    if (tid == 0) sm_abort = 0;
     grid_dependency_wait();
 
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-    const int unit = blockIdx.x, tile = unit % a.tiles, split = blockIdx.y;
-    const int64_t pair = unit / a.tiles;
-    const int b = (int)(pair / a.c.H), h = (int)(pair % a.c.H);
-    const int n = new_tokens(a.p.new_len, b, a.p.Sq);
-    const int len = a.p.kv_len ? a.p.kv_len[b] : a.c.S;
-    const int live = min(max(len, 0), a.c.S);
-
-    // rows: new token first, then the heads that share
-    int lim = 0;
+    const int per_b = a.c.H * a.tiles;                            // units of a sequence
+    // ---- the line, and this warp's run of it ----
+    const int chunk = (a.c.B + kThreads - 1) / kThreads;          // sequences of a thread
     {
-        const int row = tile * ROWS + lane, i = row / a.G;
-        if (lane < ROWS && row < a.R && i < n) {
-            lim = live;
-            if (a.p.causal) lim = (int)min((int64_t)lim, max((int64_t)len - n + i + 1, (int64_t)0));
+        int64_t mine = 0;
+        for (int b = tid * chunk; b < min((tid + 1) * chunk, a.c.B); ++b) mine += cost_of(a, b);
+        int64_t run = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, run, off);
+            if (lane >= off) run += o;
         }
-        if (warp == 0 && lane < ROWS) { sm_lim[lane] = lim; sm_i[lane] = i; }
+        if (lane == 31) sm_warp[warp] = run;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) run += sm_warp[w];
+        sm_before[tid + 1] = run;
+        if (tid == 0) sm_before[0] = 0;
+        __syncthreads();
     }
-    const int lim_max = __reduce_max_sync(0xffffffffu, lim);
-    const int lim_min = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
-
-    const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.c.k) + b * a.c.k_strides.batch + h * a.c.k_strides.head;
-    const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.c.v) + b * a.c.v_strides.batch + h * a.c.v_strides.head;
-    const float *ks = a.c.k_scale + pair * a.nb, *vs = a.c.v_scale + pair * a.nb;
-    const int32_t* list = a.p.blocks ? a.p.blocks + pair * a.p.n_blocks : nullptr;
-    const int log_block = 31 - __clz(a.c.block), log_gpb = log_block - 4;
-    const int64_t groups = lim_max == 0 ? 0 : list ? (int64_t)a.p.n_blocks << log_gpb : (lim_max + 15) >> 4;
-    const int64_t steps = (groups + kWarps * KG - 1) / (kWarps * KG);
-
-    const uint32_t ring = smem_u32(smem) + warp * kStages * (kStepBytes + kHead);
-    const unsigned char* ring_p = smem + warp * kStages * (kStepBytes + kHead);
-    // first key of group u of this warp's part of step s; 2^31 - 1: nothing there
-    auto place = [&](int64_t s, int u) -> int {
-        const int64_t g = (s * kWarps + warp) * KG + u;
-        if (g >= groups) return 0x7fffffff;
-        if (!list) return (int)(g << 4);
-        const int blk = list[g >> log_gpb];
-        if (blk < 0 || blk >= a.nb) return 0x7fffffff;
-        return (blk << log_block) + ((int)(g & ((1 << log_gpb) - 1)) << 4);
+    const int64_t total = sm_before[kThreads];
+    const int warps = warps_of(a, total), me = warp * gridDim.x + blockIdx.x;
+    if (me >= warps) return;
+    // a sequence, a unit of it and a step of that
+    struct Cursor { int b, unit, s, steps; };
+    auto locate = [&](int64_t place) -> Cursor {                  // s < 0: in the blank before the steps
+        Cursor x;
+        int i = 0;
+#pragma unroll
+        for (int y = kThreads / 2; y > 0; y >>= 1)
+            if (sm_before[i + y] <= place) i += y;                // the last thread whose sequences begin at or before it
+        int64_t at = sm_before[i];
+        x.b = i * chunk;
+        for (;; ++x.b) {
+            const int64_t cost = cost_of(a, x.b);
+            if (place - at < cost) break;
+            at += cost;
+        }
+        x.steps = steps_of(a, x.b);
+        x.unit = (int)((place - at) / (x.steps + kUnitCost));
+        x.s = (int)((place - at) % (x.steps + kUnitCost)) - kUnitCost;
+        return x;
     };
-    auto fetch_step = [&](int64_t s, int stage) {
-        if (s < steps) {
-            const uint32_t head = ring + stage * (kStepBytes + kHead), body = head + kHead + lane * 16;
-#pragma unroll
-            for (int u = 0; u < KG; ++u) {
-                const int pos = place(s, u);
-                if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(head + 32 + u * 4), "r"(pos) : "memory");
-                if (pos >= lim_max) continue;
-                if (lane < 2) fetch<4>(head + u * 8 + lane * 4, (lane ? vs : ks) + (pos >> log_block));
-                const uint32_t at = body + u * (St::kGroupLane / 16) * 512;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {                      // keys r, r + 8
-                    const uint8_t* row = kp + (int64_t)min(pos + r + 8 * x, lim_max - 1) * a.c.k_strides.seq;
-#pragma unroll
-                    for (int part = 0; part < St::kParts; ++part)
-                        fetch<St::kPart>(at + (x * St::kParts + part) * St::kPart / 16 * 512 + (D == 32 ? x * 8 : 0),
-                                         row + St::k_offset(c, part));
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {                      // keys 2c, 2c + 1, 2c + 8, 2c + 9
-                    const uint8_t* row = vp + (int64_t)min(pos + 2 * c + (x & 1) + 8 * (x >> 1), lim_max - 1) * a.c.v_strides.seq;
-                    const int byte = x * St::kVPart;
-                    fetch<St::kVPart>(at + D / 32 * 512 + byte / 16 * 512 + byte % 16, row + r * St::kVPart);
+    Cursor f = locate(run_begin(total, warps, me));               // what is fetched next
+    f.s = max(f.s, 0);
+    const Cursor end = locate(run_begin(total, warps, me + 1) - 1);       // the last place of the run
+    auto done = [&](const Cursor& x) { return x.b == end.b && x.unit == end.unit && x.s > end.s; };
+    if (done(f)) return;                                          // nothing but blanks
+    Cursor u = f;                                                 // what is multiplied next
+    auto next_unit = [&](Cursor& x) {
+        x.s = 0;
+        if (++x.unit == per_b) {
+            x.unit = 0;
+            do x.steps = steps_of(a, ++x.b); while (x.steps == 0);
+        }
+    };
+
+    // ---- fetching: K's and V's rows by TMA, scales (and the mask) by cp.async ----
+    const int extra = kHead + (a.p.keep_mask ? a.mask_rows * SG * 64 : 0);
+    unsigned char* ring = smem + ((1024 - (smem_u32(smem) & 1023)) & 1023);
+    unsigned char* heads = ring + kWarps * ST * kStepBytes<D> + warp * ST * extra;
+    ring += warp * ST * kStepBytes<D>;
+    const WaitCtx wc{&sm_abort, a.status};
+    const int log_block = 31 - __clz(a.c.block), log_gpb = log_block - 4;
+    const float *ksp, *vsp;                                       // of the fetched unit
+    const int32_t* list;
+    int f_live, f_h;
+    int next_blk;                                                 // this lane's entry of the list (lane: a group) for the next fetch
+    auto fetch_unit = [&]() {
+        f_h = f.unit / a.tiles;
+        const int64_t pair = (int64_t)f.b * a.c.H + f_h;
+        ksp = a.c.k_scale + pair * a.nb;
+        vsp = a.c.v_scale + pair * a.nb;
+        list = a.p.blocks ? a.p.blocks + pair * a.p.n_blocks : nullptr;
+        f_live = a.p.kv_len ? min(a.p.kv_len[f.b], a.c.S) : a.c.S;
+        // its queries are needed soon
+        const int gr = (f.unit % a.tiles) * ROWS + lane;
+        if (lane < ROWS && gr < a.R)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const T*>(a.p.q) + f.b * a.p.q_strides.batch +
+                (int64_t)(f_h * a.G + gr % a.G) * a.p.q_strides.head + (int64_t)(gr / a.G) * a.p.q_strides.seq));
+    };
+    auto look_ahead = [&]() {
+        if (!list) return;
+        const int at = (f.s * SG + min(lane, SG - 1)) >> log_gpb;
+        next_blk = at < a.p.n_blocks ? list[at] : -1;
+    };
+    auto fetch_step = [&](int stage) {
+        if (!done(f)) {
+            const uint32_t head = smem_u32(heads + stage * extra), body = smem_u32(ring + stage * kStepBytes<D>);
+            const uint32_t bar = smem_u32(&sm_bar[warp][stage]);
+            // lane g: where group g is
+            int pos = kNowhere;
+            if (lane < SG) {
+                const int g = f.s * SG + lane;
+                if (!list) pos = g << 4;
+                else if (next_blk >= 0 && next_blk < a.nb) pos = (next_blk << log_block) + ((g & ((1 << log_gpb) - 1)) << 4);
+                if (pos >= f_live) pos = kNowhere;
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(head + lane * 4), "r"(pos) : "memory");
+                if (pos != kNowhere) {
+                    fetch<4>(head + 16 + lane * 8, ksp + (pos >> log_block));
+                    fetch<4>(head + 20 + lane * 8, vsp + (pos >> log_block));
                 }
             }
+            // a copy of `box` keys begins at every (box / 16)th group
+            const bool copies = pos != kNowhere && (lane & ((a.box >> 4) - 1)) == 0;
+            const uint32_t n = __popc(__ballot_sync(0xffffffffu, copies));
+            if (lane == 0) mbar_arrive_expect_tx(bar, n * 2 * a.box * D);
+            __syncwarp();
+            if (copies) {
+                tma_load_4d(body + lane * Gr::kBytes, &k_map, bar, 0, pos, a.strides & 2 ? f_h : 0, a.strides & 1 ? f.b : 0);
+                tma_load_4d(body + (SG + lane) * Gr::kBytes, &v_map, bar, 0, pos, a.strides & 8 ? f_h : 0, a.strides & 4 ? f.b : 0);
+            }
+            if (a.p.keep_mask) {
+                const int i0 = (f.unit % a.tiles) * ROWS / a.G, rows = min(a.mask_rows, a.p.Sq - i0);
+#pragma unroll
+                for (int x = 0; x < SG / 2; ++x) {                 // 32 keys at a time
+                    const int base = __shfl_sync(0xffffffffu, pos, 2 * x + (lane >> 4));
+                    const int key = base == kNowhere ? a.c.S : base + (lane & 15);
+                    const float* src = a.p.keep_mask + ((int64_t)f.b * a.p.Sq + i0) * a.c.S + key;
+                    if (key < a.c.S)
+                        for (int i = 0; i < rows; ++i)
+                            fetch<4>(head + kHead + ((i * SG + 2 * x) * 16 + lane) * 4, src + (int64_t)i * a.c.S);
+                }
+            }
+            if (++f.s == f.steps && !done(f)) {
+                next_unit(f);
+                if (!done(f)) fetch_unit();
+            }
+            if (!done(f)) look_ahead();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    fetch_unit();
+    look_ahead();
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch_step(split + (int64_t)i * a.nsplit, i);
+    for (int i = 0; i < ST - 1; ++i) fetch_step(i);
 
-    // Q: a power of two per row, then fp16 fragments for every warp
-    for (int row = warp; row < ROWS; row += kWarps) {
-        const int gr = tile * ROWS + row;
-        const bool there = gr < a.R && gr / a.G < n;
-        const T* q = reinterpret_cast<const T*>(a.p.q) + b * a.p.q_strides.batch +
-                     (int64_t)(h * a.G + gr % a.G) * a.p.q_strides.head + (int64_t)(gr / a.G) * a.p.q_strides.seq;
-        float x[D / 32];
-        uint32_t most = 0;
+    // ---- a unit's rows: 2c and 2c + 1 of each tile of 8 are this lane's in S^T and O^T, row r in Q ----
+    float m[NT][2], inv[NT][2], e[NT][2], l[NT][2], cs[NT][2];       // inv = 2^(6 - e); cs: what a row's S is multiplied by
+    int lim[NT][2];                                               // keys below it are seen
+    int lim_min = 0;
+    float o[NT][W][4];
+    uint2 qf[kQRegs ? NT : 1][kQRegs ? kTerms : 1][kQRegs ? W : 1];
+    auto start_unit = [&]() {
+        const int tile = u.unit % a.tiles, h = u.unit / a.tiles;
+        const int n = new_tokens(a.p.new_len, u.b, a.p.Sq);
+        const int len = a.p.kv_len ? a.p.kv_len[u.b] : a.c.S, live = min(max(len, 0), a.c.S);
+        auto lim_of = [&](int row) -> int {
+            const int gr = tile * ROWS + row, i = gr / a.G;
+            if (gr >= a.R || i >= n) return 0;
+            return a.p.causal ? (int)min((int64_t)live, max((int64_t)len - n + i + 1, (int64_t)0)) : live;
+        };
+        lim_min = 0x7fffffff;
+        if constexpr (!kQRegs) __syncwarp();
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            x[i] = there ? ld_value(q + lane + 32 * i) : 0.f;
-            most = max(most, finite_abs_bits(x[i]));
-        }
-        most = __reduce_max_sync(0xffffffffu, most);
-        const int e = min(max((int)(most >> 23) - 127, -100), 120);
-        const float down = pow2(-e);
-        if (lane == 0) sm_c[row] = a.p.scale * 1.44269504f * pow2(e);
-        // the place of channel d in the fragments: lane (row % 8, c), product `word`, halves 0 .. 3
+        for (int t = 0; t < NT; ++t) {
+            const int gr = tile * ROWS + t * 8 + r;
+            const bool there = gr < a.R && gr / a.G < n;
+            const T* q = reinterpret_cast<const T*>(a.p.q) + u.b * a.p.q_strides.batch +
+                         (int64_t)(h * a.G + gr % a.G) * a.p.q_strides.head + (int64_t)(gr / a.G) * a.p.q_strides.seq;
+            float x[W][4];
+            uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int d = lane + 32 * i;
-            const int cc = D == 32 ? d >> 3 : (d & 63) >> 4;
-            const int word = D == 32 ? (d & 7) >> 2 : (d >> 6) * 4 + ((d & 15) >> 2);
-            const float y = x[i] * down;
-            const __half hi = __float2half_rn(y);
-            __half* dst = reinterpret_cast<__half*>(&sm_q[row >> 3][0][word][(row & 7) * 4 + cc]) + (d & 3);
-            *dst = hi;
-            if (kTerms == 2)
-                *(reinterpret_cast<__half*>(&sm_q[row >> 3][kTerms - 1][word][(row & 7) * 4 + cc]) + (d & 3)) =
-                    __float2half_rn(y - __half2float(hi));
-        }
-    }
-    __syncthreads();
-    uint2 qf[kQRegs ? NT : 1][kQRegs ? kTerms : 1][kQRegs ? MTD : 1];
-    if constexpr (kQRegs) {
+            for (int w = 0; w < W; ++w) {
+                if (there) load4(q + Gr::k_dim(c, w), a.vec_q != 0, x[w]);
+                else x[w][0] = x[w][1] = x[w][2] = x[w][3] = 0.f;
+            }
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-            for (int x = 0; x < kTerms; ++x)
+                for (int y = 0; y < 4; ++y) most = max(most, finite_abs_bits(x[w][y]));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int ex = min(max((int)(most >> 23) - 127, -100), 120);
+            const float down = pow2(-ex), up = a.p.scale * 1.44269504f * pow2(ex);
 #pragma unroll
-                for (int w = 0; w < MTD; ++w) qf[t][x][w] = sm_q[t][x][w][lane];
-    }
-    auto q_at = [&](int t, int x, int w) -> uint2 {
-        if constexpr (kQRegs) return qf[t][x][w];
-        else return sm_q[t][x][w][lane];
-    };
-
-    // of rows 2c and 2c + 1 of each tile of 8
-    float m[NT][2], inv[NT][2], e[NT][2], l[NT][2], cs[NT][2];       // inv = 2^(6 - e)
-    float o[NT][MTD][4];
+            for (int w = 0; w < W; ++w) {
+                float y[4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            m[t][x] = kNone; e[t][x] = 200.f; inv[t][x] = pow2(-100); l[t][x] = 0.f;
-            cs[t][x] = sm_c[t * 8 + 2 * c + x];
-        }
-#pragma unroll
-        for (int i = 0; i < MTD; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[t][i][x] = 0.f;
-    }
-    const bool clamped = a.p.score_clamp > 0.f;
-    const float clamp = a.p.score_clamp * 1.44269504f;
-    const float* mask = a.p.keep_mask ? a.p.keep_mask + (int64_t)b * a.p.Sq * a.c.S : nullptr;
-
-    auto group = [&](const unsigned char* body, int pos, float k_scale, float v_scale) {
-        // S^T
-        float s[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s[t][x] = 0.f;
-        {
-            uint32_t w[2][St::kWords];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if constexpr (D == 32) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(body + x * 8);
-                    w[x][0] = u.x; w[x][1] = u.y;
-                } else {
-#pragma unroll
-                    for (int part = 0; part < St::kParts; ++part) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(body + (x * St::kParts + part) * 512);
-                        w[x][4 * part] = u.x; w[x][4 * part + 1] = u.y; w[x][4 * part + 2] = u.z; w[x][4 * part + 3] = u.w;
-                    }
+                for (int k = 0; k < 4; ++k) y[k] = x[w][k] * down;
+                uint2 hi = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
+                if constexpr (kQRegs) qf[t][0][w] = hi;
+                else sm_q[warp][t][0][w][lane] = hi;
+                if constexpr (kTerms == 2) {
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                    hi = make_uint2(half2_bits(y[0] - f0.x, y[1] - f0.y), half2_bits(y[2] - f1.x, y[3] - f1.y));
+                    if constexpr (kQRegs) qf[t][kTerms - 1][w] = hi;
+                    else sm_q[warp][t][kTerms - 1][w][lane] = hi;
                 }
             }
 #pragma unroll
-            for (int i = 0; i < St::kWords; ++i) {
-                const uint32_t a0 = e4m3x2_to_half2(w[0][i] & 0xffffu), a2 = e4m3x2_to_half2(w[0][i] >> 16);
-                const uint32_t a1 = e4m3x2_to_half2(w[1][i] & 0xffffu), a3 = e4m3x2_to_half2(w[1][i] >> 16);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int x = 0; x < kTerms; ++x) {
-                        const uint2 q = q_at(t, x, i);
-                        mma(s[t], a0, a1, a2, a3, q.x, q.y);
-                    }
+            for (int k = 0; k < 2; ++k) {
+                cs[t][k] = __shfl_sync(0xffffffffu, up, (2 * c + k) * 4);
+                lim[t][k] = lim_of(t * 8 + 2 * c + k);
+                if (lim[t][k] > 0) lim_min = min(lim_min, lim[t][k]);
+                m[t][k] = kNone; e[t][k] = 200.f; inv[t][k] = pow2(-100); l[t][k] = 0.f;
             }
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[t][i][k] = 0.f;
         }
-        // scores in powers of two; s[t][0], [1]: key r with rows 2c, 2c + 1; [2], [3]: key r + 8
-        const bool whole = pos + 16 <= lim_min && !mask;
+        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+        if constexpr (!kQRegs) __syncwarp();
+    };
+    auto q_at = [&](int t, int x, int w) -> uint2 {
+        if constexpr (kQRegs) return qf[t][x][w];
+        else return sm_q[warp][t][x][w][lane];
+    };
+    const bool clamped = a.p.score_clamp > 0.f;
+    const float clamp = a.p.score_clamp * 1.44269504f;
+
+    // ---- a step's groups of keys, NG at a time from g0 on ----
+    const int k_at = Gr::swizzled(r, D == 32 ? c * 8 : c * 16);
+    const int v_at[2] = {Gr::swizzled(2 * c, r * (D / 8) & ~15) + (r * (D / 8) & 15), Gr::swizzled(2 * c + 1, r * (D / 8) & ~15) + (r * (D / 8) & 15)};
+    auto step = [&](int stage, int g0) {
+        const unsigned char* head = heads + stage * extra;
+        int pos[NG];
+        float k_scale[NG], v_scale[NG];
+        bool some = false, whole = !a.p.keep_mask;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int g = 0; g < NG; ++g) {
+            pos[g] = *reinterpret_cast<const int*>(head + (g0 + g) * 4);
+            const float2 sc = *reinterpret_cast<const float2*>(head + 16 + (g0 + g) * 8);
+            // a group that is not there has whatever the ring held: all of it is hidden, and its scales are not looked at
+            const bool there = pos[g] != kNowhere;
+            k_scale[g] = there ? sc.x : 1.f;
+            v_scale[g] = there ? sc.y : 1.f;
+            some |= there;
+            whole &= pos[g] <= lim_min - 16;
+        }
+        if (!some) return;
+        const unsigned char* body = ring + stage * kStepBytes<D> + g0 * Gr::kBytes;
+        float s[NG][NT][4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                s[t][x] *= cs[t][x & 1] * k_scale;
-                if (clamped) s[t][x] = s[t][x] < clamp ? s[t][x] : (s[t][x] == s[t][x] ? clamp : s[t][x]);
-            }
-        if (!whole) {
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int row = t * 8 + 2 * c + (x & 1), j = pos + r + 8 * (x >> 1);
-                    bool seen = j < sm_lim[row];
-                    if (mask && seen) seen = mask[(int64_t)sm_i[row] * a.c.S + j] != 0.f;
-                    if (!seen) s[t][x] = -INFINITY;
+                for (int x = 0; x < 4; ++x) s[g][t][x] = 0.f;
+#pragma unroll
+        for (int part = 0; part < Gr::kParts; ++part) {
+            constexpr int kWords = Gr::kWords;
+            uint32_t w[NG][2][kWords];
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const unsigned char* src = body + g * Gr::kBytes + x * 8 * D + (k_at ^ part * 64);
+                    if constexpr (D == 32) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(src);
+                        w[g][x][0] = v.x; w[g][x][1] = v.y;
+                    } else {
+                        const uint4 v = *reinterpret_cast<const uint4*>(src);
+                        w[g][x][0] = v.x; w[g][x][1] = v.y; w[g][x][2] = v.z; w[g][x][3] = v.w;
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_half2(w[g][0][i], a0, a2);
+                    codes_to_half2(w[g][1][i], a1, a3);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int x = 0; x < kTerms; ++x) {
+                            const uint2 q = q_at(t, x, part * kWords + i);
+                            mma(s[g][t], a0, a1, a2, a3, q.x, q.y);
+                        }
                 }
         }
-        float p[NT][4], f[NT][2];
-        bool high = false;
-        auto weigh = [&]() {
+        // s[g][t][0], [1]: key r of the group with rows 2c, 2c + 1; [2], [3]: key r + 8.  The scores are s ck.
+        float ck[NG][NT][2];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) f[t][x] = fminf(v_scale * inv[t][x], 1e38f);
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    p[t][x] = exp2_fast(s[t][x] - m[t][x & 1]);
-                    high |= p[t][x] > kLimit || p[t][x] * f[t][x & 1] > kLimit;
+                for (int x = 0; x < 2; ++x) ck[g][t][x] = cs[t][x] * k_scale[g];
+        if (!whole || clamped) {
+            const float* mask = reinterpret_cast<const float*>(head + kHead);
+            const int tile0 = (u.unit % a.tiles) * ROWS;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int key = r + 8 * (x >> 1), at = pos[g];
+                        float y = s[g][t][x] * ck[g][t][x & 1];
+                        if (clamped) y = y > clamp ? clamp : y;                   // (NaN stays)
+                        bool seen = at != kNowhere && at + key < lim[t][x & 1];
+                        if (a.p.keep_mask && seen)
+                            seen = mask[(((tile0 + t * 8 + 2 * c + (x & 1)) / a.G - tile0 / a.G) * SG + g0 + g) * 16 + key] != 0.f;
+                        s[g][t][x] = seen ? y : -INFINITY;
+                    }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) ck[g][t][0] = ck[g][t][1] = 1.f;
+        }
+        float p[NG][NT][4], w[NG][NT][4];
+        auto weigh = [&]() -> bool {
+            float top = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    // between bounds that no weight which counts comes near, so that 0 * f is 0 and a large p shows in w
+                    const float f[2] = {fmaxf(fminf(v_scale[g] * inv[t][0], 1e38f), 1e-24f), fmaxf(fminf(v_scale[g] * inv[t][1], 1e38f), 1e-24f)};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        p[g][t][x] = exp2_fast(fmaf(s[g][t][x], ck[g][t][x & 1], -m[t][x & 1]));
+                        w[g][t][x] = p[g][t][x] * f[x & 1];
+                        top = fmaxf(top, w[g][t][x]);
+                    }
                 }
-            }
+            return top > kLimit;
         };
-        weigh();
-        if (__any_sync(0xffffffffu, high)) {
-            const float lv = fmaxf(log2f(v_scale), -110.f);
+        if (__any_sync(0xffffffffu, weigh())) {
+            float lv[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) lv[g] = fmaxf(log2f(v_scale[g]), -110.f);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    float top = fmaxf(s[t][x], s[t][x + 2]);
+                    float top[NG];
 #pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                    const float m2 = fmaxf(m[t][x], ceilf(top));
+                    for (int g = 0; g < NG; ++g) {
+                        top[g] = fmaxf(s[g][t][x] * ck[g][t][x], s[g][t][x + 2] * ck[g][t][x]);
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) top[g] = fmaxf(top[g], __shfl_xor_sync(0xffffffffu, top[g], off));
+                    }
+                    float m2 = m[t][x];
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) m2 = fmaxf(m2, ceilf(top[g]));
                     const float before = m[t][x] == kNone ? -INFINITY : e[t][x] + (m[t][x] - m2);
-                    const float y = fmaxf(before, ceilf(top - m2 + lv));
+                    float y = before;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) y = fmaxf(y, ceilf(top[g] - m2 + lv[g]));
                     if (y > -1000.f && y < 1000.f) {              // a row that has seen a key
                         const float fo = before == -INFINITY ? 1.f : exp2_fast(before - y);
                         l[t][x] *= m[t][x] == kNone ? 1.f : exp2_fast(m[t][x] - m2);
@@ -330,312 +535,310 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv8_d
                         e[t][x] = y;
                         inv[t][x] = exp2_fast(6.f - y);
 #pragma unroll
-                        for (int i = 0; i < MTD; ++i) { o[t][i][x] *= fo; o[t][i][x + 2] *= fo; }
+                        for (int i = 0; i < W; ++i) { o[t][i][x] *= fo; o[t][i][x + 2] *= fo; }
                     }
                 }
             weigh();
         }
-        // W^T
-        uint32_t w0[NT][kTerms], w1[NT][kTerms];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float w[4];
+        for (int g = 0; g < NG; ++g) {
+            uint32_t w0[NT][kTerms], w1[NT][kTerms];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) l[t][x & 1] += p[g][t][x];
+                const uint32_t h0 = half2_bits(w[g][t][0], w[g][t][1]), h1 = half2_bits(w[g][t][2], w[g][t][3]);
+                w0[t][0] = transposed(h0); w1[t][0] = transposed(h1);
+                if constexpr (kTerms == 2) {
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                    w0[t][1] = transposed(half2_bits(w[g][t][0] - f0.x, w[g][t][1] - f0.y));
+                    w1[t][1] = transposed(half2_bits(w[g][t][2] - f1.x, w[g][t][3] - f1.y));
+                }
+            }
+            constexpr int VW = D / 32;                              // words of V per key and lane
+            uint32_t v[4][VW];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                l[t][x & 1] += p[t][x];
-                w[x] = p[t][x] * f[t][x & 1];
-            }
-            const uint32_t h0 = half2_bits(w[0], w[1]), h1 = half2_bits(w[2], w[3]);
-            w0[t][0] = transposed(h0); w1[t][0] = transposed(h1);
-            if constexpr (kTerms == 2) {
-                const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-                const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                w0[t][1] = transposed(half2_bits(w[0] - f0.x, w[1] - f0.y));
-                w1[t][1] = transposed(half2_bits(w[2] - f1.x, w[3] - f1.y));
-            }
-        }
-        // O^T
-        constexpr int VW = D / 32;                                  // words of V per key and lane
-        uint32_t v[4][VW];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int byte = x * St::kVPart;
-            const unsigned char* src = body + D / 32 * 512 + byte / 16 * 512 + byte % 16;
-            if constexpr (D == 128) {
-                const uint4 u = *reinterpret_cast<const uint4*>(src);
-                v[x][0] = u.x; v[x][1] = u.y; v[x][2] = u.z; v[x][3] = u.w;
-            } else if constexpr (D == 64) {
-                const uint2 u = *reinterpret_cast<const uint2*>(src);
-                v[x][0] = u.x; v[x][1] = u.y;
-            } else {
-                v[x][0] = *reinterpret_cast<const uint32_t*>(src);
-            }
-        }
-        if (!whole) {
-            // NaN among the values counts for the rows that see its key and for no other: it becomes zero, and a product of
-            // "is NaN" with "is seen" says whose sums it reaches.
-            uint32_t nan[4][VW];
-            uint32_t some = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    nan[x][i] = __vcmpeq4(v[x][i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                    some |= nan[x][i];
+                const unsigned char* src = body + (SG + g) * Gr::kBytes + (x >> 1) * 8 * D + v_at[x & 1];
+                if constexpr (D == 128) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(src);
+                    v[x][0] = y.x; v[x][1] = y.y; v[x][2] = y.z; v[x][3] = y.w;
+                } else if constexpr (D == 64) {
+                    const uint2 y = *reinterpret_cast<const uint2*>(src);
+                    v[x][0] = y.x; v[x][1] = y.y;
+                } else {
+                    v[x][0] = *reinterpret_cast<const uint32_t*>(src);
                 }
-            if (__any_sync(0xffffffffu, some != 0)) {
-                uint32_t i0[NT], i1[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    auto is = [&](int x) { return s[t][x] == -INFINITY ? 0.f : 1.f; };
-                    i0[t] = transposed(half2_bits(is(0), is(1)));
-                    i1[t] = transposed(half2_bits(is(2), is(3)));
-                }
-#pragma unroll
-                for (int i = 0; i < MTD; ++i) {
-                    // code 0x38 is 1
-                    auto pick = [&](int x, int half) {
-                        return e4m3x2_to_half2(__byte_perm(nan[x][i >> 1], nan[x + 1][i >> 1], (i & 1) ? (half ? 0x73 : 0x62)
-                                                                                                       : (half ? 0x51 : 0x40)) & 0x3838u);
-                    };
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float hit[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma(hit, pick(0, 0), pick(0, 1), pick(2, 0), pick(2, 1), i0[t], i1[t]);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            if (hit[x] > 0.f) o[t][i][x] = __int_as_float(0x7fc00000);
-                    }
-                }
+            }
+            if (!whole) {
+                // NaN among the values counts for the rows that see its key and for no other: it becomes zero, and a product
+                // of "is NaN" with "is seen" says whose sums it reaches.
+                uint32_t nan[4][VW], any = 0;
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) v[x][i] &= ~nan[x][i];
+                    for (int i = 0; i < VW; ++i) {
+                        nan[x][i] = __vcmpeq4(v[x][i] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        any |= nan[x][i];
+                    }
+                if (__any_sync(0xffffffffu, any != 0)) {
+                    uint32_t i0[NT], i1[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        auto is = [&](int x) { return s[g][t][x] == -INFINITY ? 0.f : 1.f; };
+                        i0[t] = transposed(half2_bits(is(0), is(1)));
+                        i1[t] = transposed(half2_bits(is(2), is(3)));
+                    }
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        // code 0x38 is 1
+                        auto pick = [&](int x, int half) {
+                            return e4m3x2_to_half2(__byte_perm(nan[x][i >> 1], nan[x + 1][i >> 1],
+                                                               (i & 1) ? (half ? 0x73 : 0x62) : (half ? 0x51 : 0x40)) & 0x3838u);
+                        };
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            float hit[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma(hit, pick(0, 0), pick(0, 1), pick(2, 0), pick(2, 1), i0[t], i1[t]);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                if (hit[x] > 0.f) o[t][i][x] = __int_as_float(0x7fc00000);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) v[x][i] &= ~nan[x][i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
+                uint32_t a0, a1, a2, a3;
+                codes_to_half2(__byte_perm(v[0][i >> 1], v[1][i >> 1], sel), a0, a1);
+                codes_to_half2(__byte_perm(v[2][i >> 1], v[3][i >> 1], sel), a2, a3);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int x = 0; x < kTerms; ++x) mma(o[t][i], a0, a1, a2, a3, w0[t][x], w1[t][x]);
             }
         }
+    };
+
+    // ---- a unit's sums leave: finished where this warp has seen all of it, else to scratch ----
+    auto end_unit = [&](bool from_start, bool to_end) {
+        const int tile = u.unit % a.tiles, h = u.unit / a.tiles;
+        const bool mine = from_start && to_end;
+        float* slot = a.partial + (int64_t)(2 * me + (to_end ? 0 : from_start ? 1 : 0)) * a.rows * (D + 4);
 #pragma unroll
-        for (int i = 0; i < MTD; ++i) {
-            const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
-            const uint32_t x0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], sel), x1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], sel);
-            const uint32_t a0 = e4m3x2_to_half2(x0 & 0xffffu), a1 = e4m3x2_to_half2(x0 >> 16);
-            const uint32_t a2 = e4m3x2_to_half2(x1 & 0xffffu), a3 = e4m3x2_to_half2(x1 >> 16);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int x = 0; x < 2; ++x) {
+                float sum = l[t][x];
 #pragma unroll
-                for (int x = 0; x < kTerms; ++x) mma(o[t][i], a0, a1, a2, a3, w0[t][x], w1[t][x]);
-        }
+                for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                const int row = t * 8 + 2 * c + x, gr = tile * ROWS + row;
+                if (gr >= a.R) continue;
+                if (mine) {
+                    const bool dead = lim[t][x] == 0 || sum == 0.f;
+                    const float by = pow2((int)e[t][x] - 6) / sum;
+                    T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
+                             (int64_t)(gr / a.G) * a.p.o_strides.seq + r * (D / 8);
+#pragma unroll
+                    for (int i = 0; i < W; i += 2) {
+                        const float y[4] = {dead ? 0.f : o[t][i][x] * by, dead ? 0.f : o[t][i][x + 2] * by,
+                                            dead ? 0.f : o[t][i + 1][x] * by, dead ? 0.f : o[t][i + 1][x + 2] * by};
+                        store4(out + 2 * i, a.vec_o != 0, y);
+                    }
+                    if (r == 0 && a.p.lse)
+                        a.p.lse[((int64_t)u.b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + gr / a.G] =
+                            dead ? -INFINITY : (m[t][x] == kNone ? 0.f : m[t][x] * 0.693147181f) + logf(sum);
+                } else {
+                    float* dst = slot + row * (D + 4);
+                    if (r == 0) *reinterpret_cast<float4*>(dst) = make_float4(m[t][x], e[t][x], sum, 0.f);
+#pragma unroll
+                    for (int i = 0; i < W; i += 2)
+                        *reinterpret_cast<float4*>(dst + 4 + r * (D / 8) + 2 * i) =
+                            make_float4(o[t][i][x], o[t][i][x + 2], o[t][i + 1][x], o[t][i + 1][x + 2]);
+                }
+            }
     };
 
     int stage = 0;
-    for (int64_t s = split; s < steps; s += a.nsplit) {
-        fetch_step(s + (int64_t)(kStages - 1) * a.nsplit, (stage + kStages - 1) % kStages);
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-        __syncwarp();                                               // the step's head is read by all lanes
-        const unsigned char* head = ring_p + stage * (kStepBytes + kHead);
-#pragma unroll
-        for (int u = 0; u < KG; ++u) {
-            const int pos = *reinterpret_cast<const int*>(head + 32 + u * 4);
-            if (pos >= lim_max) continue;
-            const float2 sc = *reinterpret_cast<const float2*>(head + u * 8);
-            group(head + kHead + lane * 16 + u * (St::kGroupLane / 16) * 512, pos, sc.x, sc.y);
+    uint32_t parity = 0;
+    bool from_start = u.s == 0;
+    start_unit();
+    while (true) {
+        fetch_step(stage == 0 ? ST - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        if (!mbar_wait_warp(smem_u32(&sm_bar[warp][stage]), parity, wc, 0x81)) {
+            // given up: what else this warp has on its way gets a last, short while
+            for (int i = 0; i < ST; ++i)
+                for (int x = 0; x < 4096 && !mbar_try_wait(smem_u32(&sm_bar[warp][i]), i < stage ? parity ^ 1 : parity); ++x) {}
+            break;
         }
+        __syncwarp();                                               // the step's head and mask are read by all lanes
+#pragma unroll
+        for (int g = 0; g < SG; g += NG) step(stage, g);
         __syncwarp();
-        stage = (stage + 1) % kStages;
+        if (++stage == ST) { stage = 0; parity ^= 1; }
+        const bool to_end = ++u.s == u.steps;
+        if (to_end || done(u)) {
+            end_unit(from_start, to_end);
+            if (done(u)) break;
+            next_unit(u);
+            if (done(u)) break;
+            from_start = true;
+            start_unit();
+        }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    grid_launch_dependents();
-
-    // ---- the warps' sums, tile by tile, then the CTAs' ----
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], off);
-            if (r == 0) {
-                const int row = t * 8 + 2 * c + x;
-                sm_m[warp][row] = m[t][x]; sm_e[warp][row] = e[t][x]; sm_l[warp][row] = l[t][x];
-            }
-        }
-    float* sm_o = reinterpret_cast<float*>(smem);                   // [kWarps][8][D], over the ring
-    float* sm_part = sm_o + kWarps * 8 * D;                         // [ROWS][D]
-    const bool alone = a.nsplit == 1;
-    const int64_t slot = (int64_t)unit * a.nsplit + split;
-    auto finish = [&](int row, int d, float sum, const Merged& g) {
-        const int gr = tile * ROWS + row;
-        if (gr >= a.R) return;
-        const bool dead = sm_lim[row] == 0 || g.L == 0.f;
-        T* out = reinterpret_cast<T*>(a.p.o) + b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
-                 (int64_t)(gr / a.G) * a.p.o_strides.seq;
-        st_value(out + d, dead ? 0.f : sum * (pow2((int)g.E - 6) / g.L));
-        if (d == 0 && a.p.lse)
-            a.p.lse[((int64_t)b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + gr / a.G] =
-                dead ? -INFINITY : (g.M == kNone ? 0.f : g.M * 0.693147181f) + logf(g.L);
-    };
-    // the references of n parts together; get(i) gives part i's
-    auto merge = [&](int parts, auto get) {
-        Merged g{kNone, -INFINITY, 0.f};
-        for (int i = 0; i < parts; ++i) g.M = fmaxf(g.M, get(i).M);
-        for (int i = 0; i < parts; ++i) {
-            const Merged x = get(i);
-            g.L += x.L * exp2_fast(x.M - g.M);
-            g.E = fmaxf(g.E, (x.M - g.M) + x.E);
-        }
-        return g;
-    };
-    __syncthreads();
-    if (threadIdx.x < ROWS) {
-        const int row = threadIdx.x;
-        sm_row[row] = merge(kWarps, [&](int i) { return Merged{sm_m[i][row], sm_e[i][row], sm_l[i][row]}; });
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (t) __syncthreads();
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int i = 0; i < MTD; ++i)
-                *reinterpret_cast<float2*>(sm_o + (warp * 8 + 2 * c + x) * D + r * (D / 8) + 2 * i) = make_float2(o[t][i][x], o[t][i][x + 2]);
-        __syncthreads();
-        for (int i = threadIdx.x; i < 8 * D; i += kThreads) {
-            const int row = t * 8 + i / D, d = i % D;
-            const Merged g = sm_row[row];
-            float sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-                sum += sm_o[w * 8 * D + i] * exp2_fast((sm_m[w][row] - g.M) + sm_e[w][row] - g.E);
-            if (alone) finish(row, d, sum, g);
-            else if (a.cluster) sm_part[row * D + d] = sum;
-            else a.partial[(slot * ROWS + row) * (D + 3) + 3 + d] = sum;
-        }
-    }
-    if (alone) return;
-    if (!a.cluster) {
-        if (threadIdx.x < ROWS) {
-            float* part = a.partial + (slot * ROWS + threadIdx.x) * (D + 3);
-            const Merged g = sm_row[threadIdx.x];
-            part[0] = g.M; part[1] = g.E; part[2] = g.L;
-        }
-        return;
-    }
-    // every CTA of the cluster finishes a share of the rows' values
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    for (int i = split * kThreads + threadIdx.x; i < ROWS * D; i += a.nsplit * kThreads) {
-        const int row = i / D;
-        const Merged g = merge(a.nsplit, [&](int k) { return *cluster.map_shared_rank(&sm_row[row], k); });
-        float sum = 0.f;
-        for (int k = 0; k < a.nsplit; ++k) {
-            const Merged x = *cluster.map_shared_rank(&sm_row[row], k);
-            sum += *cluster.map_shared_rank(sm_part + i, k) * exp2_fast((x.M - g.M) + x.E - g.E);
-        }
-        finish(row, i % D, sum, g);
-    }
-    cluster.sync();                                                 // until nobody reads this CTA's shared memory
 }
 
-// One CTA per row of a tile: the CTAs' shares from scratch.
-template <typename T>
-__global__ void __launch_bounds__(128) kv8_decode_merge_kernel(const __grid_constant__ DecodeArgs a, int rows) {
+// The warps' shares of a unit's row joined; what no warp or a single one has seen is zeros, or finished already.  One CTA per
+// row: its warps take shares in turn, a lane D/32 channels of each.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_constant__ DecodeArgs a, int tile_rows) {
+    constexpr int E = D / 32;
+    __shared__ int64_t sm_sum[2][kWarps];
+    __shared__ float sm_o[kWarps][D];
     grid_dependency_wait();
-    const int D = a.c.D, d = threadIdx.x, row = blockIdx.y, unit = blockIdx.x, tile = unit % a.tiles, gr = tile * rows + row;
-    if (gr >= a.R || d >= D) return;
-    const int64_t pair = unit / a.tiles;
-    const int b = (int)(pair / a.c.H), h = (int)(pair % a.c.H);
-    const float* part = a.partial + ((int64_t)unit * a.nsplit * rows + row) * (D + 3);
-    const int64_t next = (int64_t)rows * (D + 3);
-    float M = kNone, E = -INFINITY, L = 0.f, sum = 0.f;
-    for (int i = 0; i < a.nsplit; ++i) M = fmaxf(M, part[i * next]);
-    for (int i = 0; i < a.nsplit; ++i) E = fmaxf(E, (part[i * next] - M) + part[i * next + 1]);
-    for (int i = 0; i < a.nsplit; ++i) {
-        const float* x = part + i * next;
-        L += x[2] * exp2_fast(x[0] - M);
-        sum += x[3 + d] * exp2_fast((x[0] - M) + x[1] - E);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int unit = (int)(blockIdx.x % (unsigned)(a.c.H * a.tiles)), b = (int)(blockIdx.x / (unsigned)(a.c.H * a.tiles));
+    const int tile = unit % a.tiles, h = unit / a.tiles, row = blockIdx.y, gr = tile * tile_rows + row;
+    if (gr >= a.R) return;
+    int64_t before = 0, total = 0;
+    for (int x = tid; x < a.c.B; x += kThreads) {
+        const int64_t s = cost_of(a, x);
+        total += s;
+        if (x < b) before += s;
     }
-    // rows that are not there, or see nothing, have been given no sums that count
-    const int i = gr / a.G, n = new_tokens(a.p.new_len, b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[b] : a.c.S;
-    const bool dead = i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0) || len <= 0 || L == 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, off);
+        before += __shfl_xor_sync(0xffffffffu, before, off);
+    }
+    if (lane == 0) { sm_sum[0][warp] = total; sm_sum[1][warp] = before; }
+    __syncthreads();
+    total = before = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) { total += sm_sum[0][w]; before += sm_sum[1][w]; }
+    const int steps = steps_of(a, b), i = gr / a.G;
     T* out = reinterpret_cast<T*>(a.p.o) + b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
              (int64_t)i * a.p.o_strides.seq;
-    st_value(out + d, dead ? 0.f : sum * (pow2((int)E - 6) / L));
-    if (d == 0 && a.p.lse)
-        a.p.lse[((int64_t)b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + i] = dead ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
+    float* lse = a.p.lse ? a.p.lse + ((int64_t)b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + i : nullptr;
+    const int n = new_tokens(a.p.new_len, b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[b] : a.c.S;
+    if (steps == 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
+        if (tid < D) st_value(out + tid, 0.f);
+        if (tid == 0 && lse) *lse = -INFINITY;
+        return;
+    }
+    const int64_t s0 = before + (int64_t)unit * (steps + kUnitCost) + kUnitCost;       // its first step's place
+    const int warps = warps_of(a, total), w0 = warp_of(total, warps, s0), w1 = warp_of(total, warps, s0 + steps - 1);
+    if (w0 == w1) return;
+    const int parts = w1 - w0 + 1;
+    // the first share is the last thing that its warp did, the others the first
+    auto part = [&](int k) { return a.partial + ((int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * a.rows + row) * (D + 4); };
+    float M = kNone, L = 0.f, top = -INFINITY;
+    for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[0]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    for (int k = lane; k < parts; k += 32) {
+        const float4 x = *reinterpret_cast<const float4*>(part(k));
+        L += x.z * exp2_fast(x.x - M);
+        top = fmaxf(top, (x.x - M) + x.y);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        L += __shfl_xor_sync(0xffffffffu, L, off);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    float sum[E];
+#pragma unroll
+    for (int x = 0; x < E; ++x) sum[x] = 0.f;
+#pragma unroll 4
+    for (int k = warp; k < parts; k += kWarps) {
+        const float* src = part(k);
+        const float by = exp2_fast((src[0] - M) + src[1] - top);
+#pragma unroll
+        for (int x = 0; x < E; ++x) sum[x] = fmaf(src[4 + lane + 32 * x], by, sum[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < E; ++x) sm_o[warp][lane + 32 * x] = sum[x];
+    __syncthreads();
+    if (tid < D) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) y += sm_o[w][tid];
+        st_value(out + tid, L == 0.f ? 0.f : y * (pow2((int)top - 6) / L));
+    }
+    if (tid == 0 && lse) *lse = L == 0.f ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
 }
 
 // How a call is cut up; a function of the problem alone, so that the size query and the launch agree.
-struct Plan { int nt, tiles, nsplit; bool cluster; };
+struct Plan { int nt, tiles, rows, warps; };
 Plan plan_of(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     const int R = p->Hq / c->H * p->Sq;
     Plan s;
-    s.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
+    s.nt = R <= 8 ? 1 : R <= 16 || most_tiles(elem_size(p->dtype), c->D) == 2 ? 2 : 4;
     s.tiles = (R + 8 * s.nt - 1) / (8 * s.nt);
-    s.nsplit = 1;
-    s.cluster = false;
+    s.rows = R < 8 * s.nt ? R : 8 * s.nt;
     const int64_t units = (int64_t)c->B * c->H * s.tiles;
     int64_t keys = c->S;
-    if (p->blocks && (int64_t)p->n_blocks * c->block < keys) keys = (int64_t)p->n_blocks * c->block;
-    const int64_t steps = (keys + 16 * kWarps * 128 / c->D - 1) / (16 * kWarps * 128 / c->D);
-    // four CTAs per SM, each with at least two steps; more of them where the sequences may differ in length
-    const int64_t full = 4 * (int64_t)kPlanSms;
-    const int64_t want = (full + units - 1) / units, cap = (steps + 1) / 2;
-    int64_t n = want < cap ? want : cap;
-    if (units * n >= full && steps / n >= 32) n *= 4;
-    if (n > kMaxCluster && units * kMaxCluster < full) {
-        s.nsplit = (int)(n < 128 ? n : 128);
-        return s;
-    }
-    while (s.nsplit * 2 <= n && s.nsplit < kMaxCluster) s.nsplit *= 2;
-    s.cluster = s.nsplit > 1;
+    if (p->blocks) keys = (int64_t)(p->n_blocks > 1 ? p->n_blocks : 1) * c->block;
+    const int sg = step_groups(c->D);
+    const int64_t want = (units * ((keys + 16 * sg - 1) / (16 * sg) + kUnitCost) + kMinCost - 1) / kMinCost;
+    const int64_t full = (int64_t)kPlanSms * kWarps * ctas_per_sm(c->D, s.nt);
+    s.warps = (int)(want < full ? want : full);
     return s;
+}
+size_t partial_bytes(const ltca_kv8_cache* c, const Plan& s) {
+    return align_up((size_t)2 * s.warps * s.rows * (c->D + 4) * sizeof(float), 256);
+}
+
+// Keys or values as TMA sees them: [B, H, S, D] bytes, `box` keys a copy.
+int make_map(ltca_ctx* ctx, CUtensorMap* map, const void* base, const ltca_strides& st, const DecodeArgs& a, int own) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return fail(ctx, LTCA_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+    const int64_t limit = (int64_t)1 << 40;
+    if (st.seq < 0 || st.head < 0 || st.batch < 0 || st.seq >= limit || st.head >= limit || st.batch >= limit || (st.seq == 0 && a.c.S > 1))
+        return fail(ctx, LTCA_ERR_UNSUPPORTED, "decode needs a cache whose strides are between 0 (tokens: 16) and 2^40 bytes");
+    // a stride that moves nothing is not told: its extent is one, and the coordinate stays 0
+    const cuuint64_t dims[4] = {(cuuint64_t)a.c.D, (cuuint64_t)a.c.S, (cuuint64_t)(own & 2 ? a.c.H : 1), (cuuint64_t)(own & 1 ? a.c.B : 1)};
+    const cuuint64_t strides[3] = {(cuuint64_t)(a.c.S > 1 ? st.seq : 16), (cuuint64_t)(own & 2 ? st.head : 16), (cuuint64_t)(own & 1 ? st.batch : 16)};
+    const cuuint32_t box[4] = {(cuuint32_t)a.c.D, (cuuint32_t)a.box, 1, 1}, steps[4] = {1, 1, 1, 1};
+    const CUtensorMapSwizzle swizzle = a.c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : a.c.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    const CUresult rc = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, steps,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? LTCA_OK : fail(ctx, LTCA_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)rc);
 }
 
 template <typename T, int D, int NT>
 int launch(ltca_ctx* ctx, const DecodeArgs& a) {
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)((int64_t)a.c.B * a.c.H * a.tiles), a.nsplit);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kWarps * kStages * (kStepBytes + kHead);
-    static_assert(kWarps * 8 * 128 * 4 + 32 * 128 * 4 <= kWarps * kStages * (kStepBytes + kHead), "the merge lies over the ring");
-    cfg.stream = ctx->stream;
+    CUtensorMap k_map, v_map;
+    if (int rc = make_map(ctx, &k_map, a.c.k, a.c.k_strides, a, a.strides)) return rc;
+    if (int rc = make_map(ctx, &v_map, a.c.v, a.c.v_strides, a, a.strides >> 2)) return rc;
+    const int extra = kHead + (a.p.keep_mask ? a.mask_rows * kGroups<D> * 64 : 0);
+    const int bytes = 1024 + kWarps * kStages<D> * (kStepBytes<D> + extra);
+    constexpr int most = 1024 + kWarps * kStages<D> * (kStepBytes<D> + kHead + 8 * NT * kGroups<D> * 64);     // a mask row for every row
     static SmemOptIn once;
-    LTCA_CUDA_OK(ctx, opt_in_dynamic_smem(once, ctx->device, kv8_decode_kernel<T, D, NT>, (int)cfg.dynamicSmemBytes));
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 1;
-    attr[1].val.clusterDim.y = (unsigned)a.nsplit;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = a.cluster ? 2 : 1;
-    if (a.cluster && a.nsplit > 8) {
-        static SmemOptIn wide;      // clusters of more than eight CTAs are an opt-in of a kernel on one device
-        const uint64_t bit = (ctx->device >= 0 && ctx->device < 64) ? (1ull << ctx->device) : 0ull;
-        if (!bit || !(wide.done.load(std::memory_order_acquire) & bit)) {
-            LTCA_CUDA_OK(ctx, cudaFuncSetAttribute(kv8_decode_kernel<T, D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            wide.done.fetch_or(bit, std::memory_order_release);
-        }
-    }
-    LTCA_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kv8_decode_kernel<T, D, NT>, a));
+    LTCA_CUDA_OK(ctx, opt_in_dynamic_smem(once, ctx->device, kv8_decode_kernel<T, D, NT>, most));
+    const dim3 grid((unsigned)((a.warps + kWarps - 1) / kWarps));
+    LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_kernel<T, D, NT>, grid, dim3(kThreads), bytes, ctx->stream, a, k_map, v_map));
+    const dim3 rows((unsigned)((int64_t)a.c.B * a.c.H * a.tiles), (unsigned)a.rows);
+    LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_join_kernel<T, D>, dim3(rows), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
     return LTCA_OK;
 }
 template <typename T, int D>
 int launch_rows(ltca_ctx* ctx, const DecodeArgs& a, int nt) {
-    return nt == 1 ? launch<T, D, 1>(ctx, a) : nt == 2 ? launch<T, D, 2>(ctx, a) : launch<T, D, 4>(ctx, a);
+    if constexpr (most_tiles(sizeof(T), D) == 4)
+        if (nt == 4) return launch<T, D, 4>(ctx, a);
+    return nt == 1 ? launch<T, D, 1>(ctx, a) : launch<T, D, 2>(ctx, a);
 }
 template <typename T>
-int launch_width(ltca_ctx* ctx, const DecodeArgs& a, const Plan& s) {
-    int rc = a.c.D == 32 ? launch_rows<T, 32>(ctx, a, s.nt) : a.c.D == 64 ? launch_rows<T, 64>(ctx, a, s.nt) : launch_rows<T, 128>(ctx, a, s.nt);
-    if (rc || a.cluster || a.nsplit == 1) return rc;
-    const dim3 grid((unsigned)((int64_t)a.c.B * a.c.H * a.tiles), 8 * s.nt);
-    LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_merge_kernel<T>, grid, dim3(128), 0, ctx->stream, a, 8 * s.nt));
-    return LTCA_OK;
-}
-
-size_t partial_bytes(const ltca_kv8_cache* c, const Plan& s) {
-    if (s.nsplit == 1 || s.cluster) return 0;
-    return align_up((size_t)c->B * c->H * s.tiles * s.nsplit * 8 * s.nt * (c->D + 3) * sizeof(float), 256);
+int launch_width(ltca_ctx* ctx, const DecodeArgs& a, int nt) {
+    return a.c.D == 32 ? launch_rows<T, 32>(ctx, a, nt) : a.c.D == 64 ? launch_rows<T, 64>(ctx, a, nt) : launch_rows<T, 128>(ctx, a, nt);
 }
 
 }  // namespace
@@ -645,12 +848,33 @@ size_t kv8_decode_workspace(const ltca_kv8_cache* c, const ltca_kv8_decode_param
 int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     const Plan s = plan_of(c, p);
     if ((int64_t)c->B * c->H * s.tiles > 0x7fffffff) return fail(ctx, LTCA_ERR_INVALID, "too many rows of queries for one call");
-    DecodeArgs a{*c, *p, (c->S + c->block - 1) / c->block, p->Hq / c->H, p->Hq / c->H * p->Sq, s.tiles, s.nsplit, s.cluster, nullptr};
-    if (const size_t need = partial_bytes(c, s)) {
-        if (!p->workspace || p->workspace_bytes < need) return fail(ctx, LTCA_ERR_WORKSPACE, "decode needs %zu bytes of workspace", need);
-        a.partial = reinterpret_cast<float*>(p->workspace);
-    }
-    return p->dtype == LTCA_BF16 ? launch_width<__nv_bfloat16>(ctx, a, s) : launch_width<float>(ctx, a, s);
+    if (p->blocks && (int64_t)p->n_blocks * c->block > (1 << 30))
+        return fail(ctx, LTCA_ERR_UNSUPPORTED, "the listed blocks hold more than 2^30 tokens");
+    DecodeArgs a;
+    memset(&a, 0, sizeof(a));
+    a.c = *c; a.p = *p;
+    a.nb = (c->S + c->block - 1) / c->block;
+    a.G = p->Hq / c->H;
+    a.R = a.G * p->Sq;
+    a.tiles = s.tiles; a.rows = s.rows; a.warps = s.warps;
+    const int es = elem_size(p->dtype);
+    auto on = [&](const void* ptr, const ltca_strides& st, int to) {
+        return !((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(st.batch * es) | (uintptr_t)(st.head * es) | (uintptr_t)(st.seq * es)) & (to - 1));
+    };
+    a.vec_q = on(p->q, p->q_strides, 4 * es);
+    a.vec_o = on(p->o, p->o_strides, 4 * es);
+    // new tokens that 8 NT rows in a line reach
+    const int span = (8 * s.nt - 1 + a.G - 1) / a.G + 1;
+    a.mask_rows = span < p->Sq ? span : p->Sq;
+    a.box = 16 * step_groups(c->D);
+    if (p->blocks && c->block < a.box) a.box = c->block;
+    a.strides = (c->B > 1 && c->k_strides.batch ? 1 : 0) | (c->H > 1 && c->k_strides.head ? 2 : 0) |
+                (c->B > 1 && c->v_strides.batch ? 4 : 0) | (c->H > 1 && c->v_strides.head ? 8 : 0);
+    a.status = ctx->d_status;
+    const size_t need = partial_bytes(c, s);
+    if (!p->workspace || p->workspace_bytes < need) return fail(ctx, LTCA_ERR_WORKSPACE, "decode needs %zu bytes of workspace", need);
+    a.partial = reinterpret_cast<float*>(p->workspace);
+    return p->dtype == LTCA_BF16 ? launch_width<__nv_bfloat16>(ctx, a, s.nt) : launch_width<float>(ctx, a, s.nt);
 }
 
 }  // namespace ltca
