@@ -22,8 +22,12 @@
 //
 // Every warp works for itself.  The steps of all units (a pair and up to 8 NT of its rows) lie in one line, each unit's behind
 // a blank that stands for what a unit costs beside them, and a warp takes an equal run of it, whatever the lengths; it fetches
-// across the borders of units, so that the stream does not stop while a unit's queries are brought in or its sums leave.  A unit that one warp has seen whole is finished by it; shares
-// of a unit go to scratch and are joined by a second kernel.
+// across the borders of units, so that the stream does not stop while a unit's queries are brought in or its sums leave.  A
+// unit that one warp has seen whole is finished by it; shares of a unit go to scratch and are joined by a second kernel.
+// Calls that are over in a few steps take no line: the CTAs of a cluster divide a unit's steps and join their shares through
+// each other's shared memory, in one launch.
+#include <cooperative_groups.h>
+
 #include "kv8.cuh"
 
 namespace ltca {
@@ -33,6 +37,8 @@ namespace {
 constexpr int kWarps = 4;                   // of a CTA
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHead = 48;                   // a step's positions and scales
+constexpr int kMaxCluster = 16;             // CTAs that join their shares through shared memory
+constexpr int kClusterSteps = 8;            // of a warp there, at most
 constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do
 constexpr int kUnitCost = 2;                // what a unit costs beside its steps, in steps
 constexpr int kNowhere = 0x7fffffff;        // the position of a group that is not there
@@ -60,6 +66,7 @@ struct DecodeArgs {
     int mask_rows;              // rows of keep_mask that a tile's rows need
     int box;                    // keys of a copy
     int strides;                // what has a stride of its own: sequences of k (1) and v (4), heads of k (2) and v (8)
+    int splits;                 // CTAs (a cluster) of a unit; 0: the warps share one line
     float* partial;             // [2 warps][rows][D + 4]
     uint32_t* status;
 };
@@ -80,8 +87,11 @@ __device__ __forceinline__ int64_t cost_of(const DecodeArgs& a, int b) {        
 __device__ __forceinline__ int warps_of(const DecodeArgs& a, int64_t total) {
     return (int)min((int64_t)a.warps, (total + kMinCost - 1) / kMinCost);
 }
-__device__ __forceinline__ int64_t run_begin(int64_t total, int warps, int w) { return total * w / warps; }
-__device__ __forceinline__ int warp_of(int64_t total, int warps, int64_t at) { return (int)(((at + 1) * warps - 1) / total); }
+__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {                            // neither below zero
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+__device__ __forceinline__ int64_t run_begin(int64_t total, int warps, int w) { return divided(total * w, warps); }
+__device__ __forceinline__ int warp_of(int64_t total, int warps, int64_t at) { return (int)divided((at + 1) * warps - 1, total); }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -164,6 +174,48 @@ struct Group {
     static __device__ __forceinline__ int k_dim(int c, int w) { return D == 32 ? c * 8 + 4 * w : (w >> 2) * 64 + c * 16 + 4 * (w & 3); }
 };
 
+// The shares of a row joined by a CTA: its warps take shares in turn, a lane D/32 channels of each.  part(k): share k's m, e, l
+// and its sums behind them.
+template <typename T, int D, typename Part>
+__device__ __forceinline__ void join_row(int parts, Part part, float (&sm_o)[kWarps][D], T* out, float* lse) {
+    constexpr int E = D / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float M = kNone, L = 0.f, top = -INFINITY;
+    for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[0]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    for (int k = lane; k < parts; k += 32) {
+        const float4 x = *reinterpret_cast<const float4*>(part(k));
+        L += x.z * exp2_fast(x.x - M);
+        top = fmaxf(top, (x.x - M) + x.y);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        L += __shfl_xor_sync(0xffffffffu, L, off);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    float sum[E];
+#pragma unroll
+    for (int x = 0; x < E; ++x) sum[x] = 0.f;
+#pragma unroll 4
+    for (int k = warp; k < parts; k += kWarps) {
+        const float* src = part(k);
+        const float by = exp2_fast((src[0] - M) + src[1] - top);
+#pragma unroll
+        for (int x = 0; x < E; ++x) sum[x] = fmaf(src[4 + lane + 32 * x], by, sum[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < E; ++x) sm_o[warp][lane + 32 * x] = sum[x];
+    __syncthreads();
+    if (tid < D) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) y += sm_o[w][tid];
+        st_value(out + tid, L == 0.f ? 0.f : y * (pow2((int)top - 6) / L));
+    }
+    if (tid == 0 && lse) *lse = L == 0.f ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, kCtas<D, NT>)
 kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -179,6 +231,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     __shared__ int64_t sm_before[kThreads + 1];                   // the line up to each thread's sequences
     __shared__ int64_t sm_warp[kWarps];
     __shared__ uint32_t sm_abort;
+    __shared__ float sm_join[kWarps][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
     if (lane < ST) mbar_init(smem_u32(&sm_bar[warp][lane]), 1);
     mbar_fence_init();
@@ -186,12 +239,22 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     grid_dependency_wait();
 
     const int per_b = a.c.H * a.tiles;                            // units of a sequence
-    // ---- the line, and this warp's run of it ----
-    const int chunk = (a.c.B + kThreads - 1) / kThreads;          // sequences of a thread
-    {
-        int64_t mine = 0;
-        for (int b = tid * chunk; b < min((tid + 1) * chunk, a.c.B); ++b) mine += cost_of(a, b);
-        int64_t run = mine;
+    // a sequence, a unit of it and a step of that
+    struct Cursor { int b, unit, s, steps; };
+    Cursor f, end;                                                // what is fetched next; the last step of the run
+    int me = 0;
+    if (a.splits) {
+        const int unit = blockIdx.x / a.splits, parts = kWarps * a.splits, w = (blockIdx.x % a.splits) * kWarps + warp;
+        f.b = unit / per_b;
+        f.unit = unit % per_b;
+        f.steps = steps_of(a, f.b);
+        end = f;
+        f.s = (int)((uint32_t)f.steps * w / parts);
+        end.s = (int)((uint32_t)f.steps * (w + 1) / parts) - 1;
+    } else {
+        const int chunk = (a.c.B + kThreads - 1) / kThreads;      // sequences of a thread
+        int64_t run = 0;
+        for (int b = tid * chunk; b < min((tid + 1) * chunk, a.c.B); ++b) run += cost_of(a, b);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const int64_t o = __shfl_up_sync(0xffffffffu, run, off);
@@ -203,43 +266,45 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         sm_before[tid + 1] = run;
         if (tid == 0) sm_before[0] = 0;
         __syncthreads();
-    }
-    const int64_t total = sm_before[kThreads];
-    const int warps = warps_of(a, total), me = warp * gridDim.x + blockIdx.x;
-    if (me >= warps) return;
-    // a sequence, a unit of it and a step of that
-    struct Cursor { int b, unit, s, steps; };
-    auto locate = [&](int64_t place) -> Cursor {                  // s < 0: in the blank before the steps
-        Cursor x;
-        int i = 0;
+        const int64_t total = sm_before[kThreads];
+        const int warps = warps_of(a, total);
+        me = warp * gridDim.x + blockIdx.x;
+        if (me >= warps) return;
+        auto locate = [&](int64_t place) -> Cursor {              // s < 0: in the blank before the steps
+            Cursor x;
+            int i = 0;
 #pragma unroll
-        for (int y = kThreads / 2; y > 0; y >>= 1)
-            if (sm_before[i + y] <= place) i += y;                // the last thread whose sequences begin at or before it
-        int64_t at = sm_before[i];
-        x.b = i * chunk;
-        for (;; ++x.b) {
-            const int64_t cost = cost_of(a, x.b);
-            if (place - at < cost) break;
-            at += cost;
-        }
-        x.steps = steps_of(a, x.b);
-        x.unit = (int)((place - at) / (x.steps + kUnitCost));
-        x.s = (int)((place - at) % (x.steps + kUnitCost)) - kUnitCost;
-        return x;
-    };
-    Cursor f = locate(run_begin(total, warps, me));               // what is fetched next
-    f.s = max(f.s, 0);
-    const Cursor end = locate(run_begin(total, warps, me + 1) - 1);       // the last place of the run
-    auto done = [&](const Cursor& x) { return x.b == end.b && x.unit == end.unit && x.s > end.s; };
-    if (done(f)) return;                                          // nothing but blanks
+            for (int y = kThreads / 2; y > 0; y >>= 1)
+                if (sm_before[i + y] <= place) i += y;            // the last thread whose sequences begin at or before it
+            int64_t at = sm_before[i];
+            x.b = i * chunk;
+            for (;; ++x.b) {
+                const int64_t cost = cost_of(a, x.b);
+                if (place - at < cost) break;
+                at += cost;
+            }
+            x.steps = steps_of(a, x.b);
+            x.unit = (int)divided(place - at, x.steps + kUnitCost);
+            x.s = (int)(place - at - (int64_t)x.unit * (x.steps + kUnitCost)) - kUnitCost;
+            return x;
+        };
+        f = locate(run_begin(total, warps, me));
+        f.s = max(f.s, 0);
+        end = locate(run_begin(total, warps, me + 1) - 1);
+    }
+    // steps of the run in the unit that x is in
+    auto left_of = [&](const Cursor& x) -> int { return (x.b == end.b && x.unit == end.unit ? end.s + 1 : x.steps) - x.s; };
+    int f_left = left_of(f), u_left = f_left;
+    if (f_left <= 0 && !a.splits) return;                         // nothing but blanks
     Cursor u = f;                                                 // what is multiplied next
-    auto next_unit = [&](Cursor& x) {
+    auto next_unit = [&](Cursor& x) {                             // only where the run has more
         x.s = 0;
         if (++x.unit == per_b) {
             x.unit = 0;
             do x.steps = steps_of(a, ++x.b); while (x.steps == 0);
         }
     };
+    auto at_end = [&](const Cursor& x) { return x.b == end.b && x.unit == end.unit; };
 
     // ---- fetching: K's and V's rows by TMA, scales (and the mask) by cp.async ----
     const int extra = kHead + (a.p.keep_mask ? a.mask_rows * SG * 64 : 0);
@@ -248,15 +313,14 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     ring += warp * ST * kStepBytes<D>;
     const WaitCtx wc{&sm_abort, a.status};
     const int log_block = 31 - __clz(a.c.block), log_gpb = log_block - 4;
-    const float *ksp, *vsp;                                       // of the fetched unit
+    const float* sp;                                              // of the fetched unit: k's scales for even lanes, v's for odd ones
     const int32_t* list;
     int f_live, f_h;
-    int next_blk;                                                 // this lane's entry of the list (lane: a group) for the next fetch
+    int next_blk;                                                 // this lane's entry of the list (lane / 2: a group) for the next fetch
     auto fetch_unit = [&]() {
         f_h = f.unit / a.tiles;
         const int64_t pair = (int64_t)f.b * a.c.H + f_h;
-        ksp = a.c.k_scale + pair * a.nb;
-        vsp = a.c.v_scale + pair * a.nb;
+        sp = (lane & 1 ? a.c.v_scale : a.c.k_scale) + pair * a.nb;
         list = a.p.blocks ? a.p.blocks + pair * a.p.n_blocks : nullptr;
         f_live = a.p.kv_len ? min(a.p.kv_len[f.b], a.c.S) : a.c.S;
         // its queries are needed soon
@@ -266,41 +330,44 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 (int64_t)(f_h * a.G + gr % a.G) * a.p.q_strides.head + (int64_t)(gr / a.G) * a.p.q_strides.seq));
     };
     auto look_ahead = [&]() {
-        if (!list) return;
-        const int at = (f.s * SG + min(lane, SG - 1)) >> log_gpb;
+        const int at = (f.s * SG + min(lane >> 1, SG - 1)) >> log_gpb;
         next_blk = at < a.p.n_blocks ? list[at] : -1;
     };
     auto fetch_step = [&](int stage) {
-        if (!done(f)) {
+        if (f_left > 0) {
             const uint32_t head = smem_u32(heads + stage * extra), body = smem_u32(ring + stage * kStepBytes<D>);
             const uint32_t bar = smem_u32(&sm_bar[warp][stage]);
-            // lane g: where group g is
+            // lanes 2g and 2g + 1: where group g is
             int pos = kNowhere;
-            if (lane < SG) {
-                const int g = f.s * SG + lane;
+            if (lane < 2 * SG) {
+                const int g = f.s * SG + (lane >> 1);
                 if (!list) pos = g << 4;
                 else if (next_blk >= 0 && next_blk < a.nb) pos = (next_blk << log_block) + ((g & ((1 << log_gpb) - 1)) << 4);
                 if (pos >= f_live) pos = kNowhere;
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(head + lane * 4), "r"(pos) : "memory");
-                if (pos != kNowhere) {
-                    fetch<4>(head + 16 + lane * 8, ksp + (pos >> log_block));
-                    fetch<4>(head + 20 + lane * 8, vsp + (pos >> log_block));
-                }
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(head + (lane >> 1) * 4), "r"(pos) : "memory");
+                if (pos != kNowhere) fetch<4>(head + 16 + lane * 4, sp + (pos >> log_block));
             }
-            // a copy of `box` keys begins at every (box / 16)th group
-            const bool copies = pos != kNowhere && (lane & ((a.box >> 4) - 1)) == 0;
-            const uint32_t n = __popc(__ballot_sync(0xffffffffu, copies));
-            if (lane == 0) mbar_arrive_expect_tx(bar, n * 2 * a.box * D);
-            __syncwarp();
-            if (copies) {
-                tma_load_4d(body + lane * Gr::kBytes, &k_map, bar, 0, pos, a.strides & 2 ? f_h : 0, a.strides & 1 ? f.b : 0);
-                tma_load_4d(body + (SG + lane) * Gr::kBytes, &v_map, bar, 0, pos, a.strides & 8 ? f_h : 0, a.strides & 4 ? f.b : 0);
+            if (!list) {                                          // one copy
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar, kStepBytes<D>);
+                    tma_load_4d(body, &k_map, bar, 0, pos, a.strides & 2 ? f_h : 0, a.strides & 1 ? f.b : 0);
+                    tma_load_4d(body + SG * Gr::kBytes, &v_map, bar, 0, pos, a.strides & 8 ? f_h : 0, a.strides & 4 ? f.b : 0);
+                }
+            } else {                                              // one for every `box` keys
+                const bool copies = pos != kNowhere && (lane & ((a.box >> 3) - 1)) == 0;
+                const uint32_t n = __popc(__ballot_sync(0xffffffffu, copies));
+                if (lane == 0) mbar_arrive_expect_tx(bar, n * 2 * a.box * D);
+                __syncwarp();
+                if (copies) {
+                    tma_load_4d(body + (lane >> 1) * Gr::kBytes, &k_map, bar, 0, pos, a.strides & 2 ? f_h : 0, a.strides & 1 ? f.b : 0);
+                    tma_load_4d(body + (SG + (lane >> 1)) * Gr::kBytes, &v_map, bar, 0, pos, a.strides & 8 ? f_h : 0, a.strides & 4 ? f.b : 0);
+                }
             }
             if (a.p.keep_mask) {
                 const int i0 = (f.unit % a.tiles) * ROWS / a.G, rows = min(a.mask_rows, a.p.Sq - i0);
 #pragma unroll
                 for (int x = 0; x < SG / 2; ++x) {                 // 32 keys at a time
-                    const int base = __shfl_sync(0xffffffffu, pos, 2 * x + (lane >> 4));
+                    const int base = __shfl_sync(0xffffffffu, pos, 4 * x + 2 * (lane >> 4));
                     const int key = base == kNowhere ? a.c.S : base + (lane & 15);
                     const float* src = a.p.keep_mask + ((int64_t)f.b * a.p.Sq + i0) * a.c.S + key;
                     if (key < a.c.S)
@@ -308,16 +375,20 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                             fetch<4>(head + kHead + ((i * SG + 2 * x) * 16 + lane) * 4, src + (int64_t)i * a.c.S);
                 }
             }
-            if (++f.s == f.steps && !done(f)) {
+            ++f.s;
+            if (--f_left == 0 && !at_end(f)) {
                 next_unit(f);
-                if (!done(f)) fetch_unit();
+                f_left = left_of(f);
+                if (f_left > 0) fetch_unit();
             }
-            if (!done(f)) look_ahead();
+            if (list && f_left > 0) look_ahead();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    fetch_unit();
-    look_ahead();
+    if (f_left > 0) {
+        fetch_unit();
+        if (list) look_ahead();
+    }
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) fetch_step(i);
 
@@ -327,6 +398,19 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     int lim_min = 0;
     float o[NT][W][4];
     uint2 qf[kQRegs ? NT : 1][kQRegs ? kTerms : 1][kQRegs ? W : 1];
+    uint64_t mask_row = 0;                                        // the mask's rows of this lane's rows, a byte each
+    int mask_rows = 0;                                            // that the tile's rows need
+    auto clear = [&]() {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) { m[t][k] = kNone; e[t][k] = 200.f; inv[t][k] = pow2(-100); l[t][k] = 0.f; }
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[t][i][k] = 0.f;
+        }
+    };
     auto start_unit = [&]() {
         const int tile = u.unit % a.tiles, h = u.unit / a.tiles;
         const int n = new_tokens(a.p.new_len, u.b, a.p.Sq);
@@ -380,14 +464,19 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 cs[t][k] = __shfl_sync(0xffffffffu, up, (2 * c + k) * 4);
                 lim[t][k] = lim_of(t * 8 + 2 * c + k);
                 if (lim[t][k] > 0) lim_min = min(lim_min, lim[t][k]);
-                m[t][k] = kNone; e[t][k] = 200.f; inv[t][k] = pow2(-100); l[t][k] = 0.f;
             }
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[t][i][k] = 0.f;
         }
+        clear();
         lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+        if (a.p.keep_mask) {
+            const int tile0 = tile * ROWS;
+            mask_row = 0;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) mask_row |= (uint64_t)(min((tile0 + t * 8 + 2 * c + k) / a.G - tile0 / a.G, 31)) << (8 * (2 * t + k));
+            mask_rows = min(a.mask_rows, a.p.Sq - tile0 / a.G);
+        }
         if constexpr (!kQRegs) __syncwarp();
     };
     auto q_at = [&](int t, int x, int w) -> uint2 {
@@ -404,7 +493,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         const unsigned char* head = heads + stage * extra;
         int pos[NG];
         float k_scale[NG], v_scale[NG];
-        bool some = false, whole = !a.p.keep_mask;
+        bool some = false, whole = true;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             pos[g] = *reinterpret_cast<const int*>(head + (g0 + g) * 4);
@@ -417,6 +506,26 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
             whole &= pos[g] <= lim_min - 16;
         }
         if (!some) return;
+        // The mask as words, bit = key (of the step's 32 that these groups are among): lane i has the word of its row i.  What
+        // hides or shows all of a step's keys from all rows is settled here.
+        uint32_t word = 0xffffffffu;
+        if (a.p.keep_mask) {
+            const float* mask = reinterpret_cast<const float*>(head + kHead) + (g0 & ~1) * 16 + lane;
+            uint32_t any = 0, all = 0xffffffffu;
+            for (int i = 0; i < mask_rows; ++i) {
+                const uint32_t v = __ballot_sync(0xffffffffu, mask[i * SG * 16] != 0.f);
+                if (lane == i) word = v;
+                any |= v;
+                all &= v;
+            }
+            const uint32_t those = NG == 2 ? 0xffffffffu : 0xffffu << (16 * (g0 & 1));
+            uint32_t seen = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                if (pos[g] != kNowhere) seen |= 0xffffu << (16 * ((g0 + g) & 1));
+            if ((any & seen) == 0) return;
+            if ((all & those) != those) whole = false;
+        }
         const unsigned char* body = ring + stage * kStepBytes<D> + g0 * Gr::kBytes;
         float s[NG][NT][4];
 #pragma unroll
@@ -467,20 +576,23 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
                 for (int x = 0; x < 2; ++x) ck[g][t][x] = cs[t][x] * k_scale[g];
         if (!whole || clamped) {
-            const float* mask = reinterpret_cast<const float*>(head + kHead);
-            const int tile0 = (u.unit % a.tiles) * ROWS;
+            uint32_t bits[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    bits[t][x] = __shfl_sync(0xffffffffu, word, (int)(mask_row >> (8 * (2 * t + x))) & 31) >> r;
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const int key = r + 8 * (x >> 1), at = pos[g];
+                        const int key = 8 * (x >> 1);
                         float y = s[g][t][x] * ck[g][t][x & 1];
                         if (clamped) y = y > clamp ? clamp : y;                   // (NaN stays)
-                        bool seen = at != kNowhere && at + key < lim[t][x & 1];
-                        if (a.p.keep_mask && seen)
-                            seen = mask[(((tile0 + t * 8 + 2 * c + (x & 1)) / a.G - tile0 / a.G) * SG + g0 + g) * 16 + key] != 0.f;
+                        const bool seen = pos[g] != kNowhere && pos[g] + r + key < lim[t][x & 1] &&
+                                          (bits[t][x & 1] >> (16 * ((g0 + g) & 1) + key) & 1);
                         s[g][t][x] = seen ? y : -INFINITY;
                     }
 #pragma unroll
@@ -627,10 +739,8 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     };
 
     // ---- a unit's sums leave: finished where this warp has seen all of it, else to scratch ----
-    auto end_unit = [&](bool from_start, bool to_end) {
+    auto end_unit = [&](bool mine, float* slot) {
         const int tile = u.unit % a.tiles, h = u.unit / a.tiles;
-        const bool mine = from_start && to_end;
-        float* slot = a.partial + (int64_t)(2 * me + (to_end ? 0 : from_start ? 1 : 0)) * a.rows * (D + 4);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -668,8 +778,9 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     int stage = 0;
     uint32_t parity = 0;
     bool from_start = u.s == 0;
-    start_unit();
-    while (true) {
+    if (u_left > 0) start_unit();
+    else clear();
+    while (u_left > 0) {
         fetch_step(stage == 0 ? ST - 1 : stage - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
         if (!mbar_wait_warp(smem_u32(&sm_bar[warp][stage]), parity, wc, 0x81)) {
@@ -683,24 +794,53 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         for (int g = 0; g < SG; g += NG) step(stage, g);
         __syncwarp();
         if (++stage == ST) { stage = 0; parity ^= 1; }
-        const bool to_end = ++u.s == u.steps;
-        if (to_end || done(u)) {
-            end_unit(from_start, to_end);
-            if (done(u)) break;
-            next_unit(u);
-            if (done(u)) break;
-            from_start = true;
-            start_unit();
-        }
+        ++u.s;
+        if (--u_left > 0 || a.splits) continue;
+        const bool to_end = u.s == u.steps;
+        end_unit(from_start && to_end, a.partial + (int64_t)(2 * me + (to_end ? 0 : from_start ? 1 : 0)) * a.rows * (D + 4));
+        if (at_end(u)) break;
+        next_unit(u);
+        u_left = left_of(u);
+        if (u_left <= 0) break;
+        from_start = true;
+        start_unit();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!a.splits) return;
+
+    // ---- the cluster's shares, over the rings; its CTAs take the rows in turn ----
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    float* share = reinterpret_cast<float*>(ring - warp * ST * kStepBytes<D>);
+    __syncthreads();
+    end_unit(false, share + warp * a.rows * (D + 4));
+    if (a.splits > 1) cluster.sync();
+    else __syncthreads();
+    const int tile = u.unit % a.tiles, h = u.unit / a.tiles, rank = blockIdx.x % a.splits;
+    const int n = new_tokens(a.p.new_len, u.b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[u.b] : a.c.S;
+    for (int row = rank; row < ROWS && tile * ROWS + row < a.R; row += a.splits) {
+        const int gr = tile * ROWS + row, i = gr / a.G;
+        T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
+                 (int64_t)i * a.p.o_strides.seq;
+        float* lse = a.p.lse ? a.p.lse + ((int64_t)u.b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + i : nullptr;
+        if (len <= 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
+            if (tid < D) st_value(out + tid, 0.f);
+            if (tid == 0 && lse) *lse = -INFINITY;
+            continue;
+        }
+        join_row<T, D>(kWarps * a.splits, [&](int k) -> const float* {
+            const float* mine = share + ((k & (kWarps - 1)) * a.rows + row) * (D + 4);
+            return a.splits > 1 ? cluster.map_shared_rank(mine, k / kWarps) : mine;
+        }, sm_join, out, lse);
+        __syncthreads();
+    }
+    if (a.splits > 1) cluster.sync();                               // until nobody reads this CTA's shared memory
 }
 
 // The warps' shares of a unit's row joined; what no warp or a single one has seen is zeros, or finished already.  One CTA per
 // row: its warps take shares in turn, a lane D/32 channels of each.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_constant__ DecodeArgs a, int tile_rows) {
-    constexpr int E = D / 32;
     __shared__ int64_t sm_sum[2][kWarps];
     __shared__ float sm_o[kWarps][D];
     grid_dependency_wait();
@@ -740,44 +880,11 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_
     const int parts = w1 - w0 + 1;
     // the first share is the last thing that its warp did, the others the first
     auto part = [&](int k) { return a.partial + ((int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * a.rows + row) * (D + 4); };
-    float M = kNone, L = 0.f, top = -INFINITY;
-    for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[0]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    for (int k = lane; k < parts; k += 32) {
-        const float4 x = *reinterpret_cast<const float4*>(part(k));
-        L += x.z * exp2_fast(x.x - M);
-        top = fmaxf(top, (x.x - M) + x.y);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        L += __shfl_xor_sync(0xffffffffu, L, off);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    }
-    float sum[E];
-#pragma unroll
-    for (int x = 0; x < E; ++x) sum[x] = 0.f;
-#pragma unroll 4
-    for (int k = warp; k < parts; k += kWarps) {
-        const float* src = part(k);
-        const float by = exp2_fast((src[0] - M) + src[1] - top);
-#pragma unroll
-        for (int x = 0; x < E; ++x) sum[x] = fmaf(src[4 + lane + 32 * x], by, sum[x]);
-    }
-#pragma unroll
-    for (int x = 0; x < E; ++x) sm_o[warp][lane + 32 * x] = sum[x];
-    __syncthreads();
-    if (tid < D) {
-        float y = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) y += sm_o[w][tid];
-        st_value(out + tid, L == 0.f ? 0.f : y * (pow2((int)top - 6) / L));
-    }
-    if (tid == 0 && lse) *lse = L == 0.f ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
+    join_row<T, D>(parts, part, sm_o, out, lse);
 }
 
 // How a call is cut up; a function of the problem alone, so that the size query and the launch agree.
-struct Plan { int nt, tiles, rows, warps; };
+struct Plan { int nt, tiles, rows, warps, splits; };
 Plan plan_of(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     const int R = p->Hq / c->H * p->Sq;
     Plan s;
@@ -788,9 +895,22 @@ Plan plan_of(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     int64_t keys = c->S;
     if (p->blocks) keys = (int64_t)(p->n_blocks > 1 ? p->n_blocks : 1) * c->block;
     const int sg = step_groups(c->D);
-    const int64_t want = (units * ((keys + 16 * sg - 1) / (16 * sg) + kUnitCost) + kMinCost - 1) / kMinCost;
-    const int64_t full = (int64_t)kPlanSms * kWarps * ctas_per_sm(c->D, s.nt);
-    s.warps = (int)(want < full ? want : full);
+    const int64_t steps = (keys + 16 * sg - 1) / (16 * sg), full = (int64_t)kPlanSms * ctas_per_sm(c->D, s.nt);
+    // One cluster a unit where all of them are on the SMs at once and no warp gets more than a few steps.
+    s.splits = 0;
+    s.warps = 0;
+    if (units <= full) {
+        int n = (int)(full / units);
+        if (n > kMaxCluster) n = kMaxCluster;
+        if (n > (steps + kWarps - 1) / kWarps) n = (int)((steps + kWarps - 1) / kWarps);
+        while (n & (n - 1)) n &= n - 1;
+        if (steps <= (int64_t)kClusterSteps * kWarps * n) {
+            s.splits = n;
+            return s;
+        }
+    }
+    const int64_t want = (units * (steps + kUnitCost) + kMinCost - 1) / kMinCost;
+    s.warps = (int)(want < full * kWarps ? want : full * kWarps);
     return s;
 }
 size_t partial_bytes(const ltca_kv8_cache* c, const Plan& s) {
@@ -820,14 +940,42 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
     if (int rc = make_map(ctx, &k_map, a.c.k, a.c.k_strides, a, a.strides)) return rc;
     if (int rc = make_map(ctx, &v_map, a.c.v, a.c.v_strides, a, a.strides >> 2)) return rc;
     const int extra = kHead + (a.p.keep_mask ? a.mask_rows * kGroups<D> * 64 : 0);
-    const int bytes = 1024 + kWarps * kStages<D> * (kStepBytes<D> + extra);
+    constexpr int shares = kWarps * 8 * NT * (D + 4) * 4;
+    const int ring = kWarps * kStages<D> * (kStepBytes<D> + extra), bytes = 1024 + (ring > shares ? ring : shares);
     constexpr int most = 1024 + kWarps * kStages<D> * (kStepBytes<D> + kHead + 8 * NT * kGroups<D> * 64);     // a mask row for every row
     static SmemOptIn once;
-    LTCA_CUDA_OK(ctx, opt_in_dynamic_smem(once, ctx->device, kv8_decode_kernel<T, D, NT>, most));
-    const dim3 grid((unsigned)((a.warps + kWarps - 1) / kWarps));
-    LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_kernel<T, D, NT>, grid, dim3(kThreads), bytes, ctx->stream, a, k_map, v_map));
-    const dim3 rows((unsigned)((int64_t)a.c.B * a.c.H * a.tiles), (unsigned)a.rows);
-    LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_join_kernel<T, D>, dim3(rows), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
+    LTCA_CUDA_OK(ctx, opt_in_dynamic_smem(once, ctx->device, kv8_decode_kernel<T, D, NT>, most > shares ? most : shares));
+    const int64_t units = (int64_t)a.c.B * a.c.H * a.tiles;
+    if (!a.splits) {
+        const dim3 grid((unsigned)((a.warps + kWarps - 1) / kWarps));
+        LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_kernel<T, D, NT>, grid, dim3(kThreads), bytes, ctx->stream, a, k_map, v_map));
+        LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_join_kernel<T, D>, dim3((unsigned)units, (unsigned)a.rows), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
+        return LTCA_OK;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(units * a.splits));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.splits > 1 ? 2 : 1;
+    if (a.splits > 8) {
+        static SmemOptIn wide;      // clusters of more than eight CTAs are an opt-in of a kernel on one device
+        const uint64_t bit = (ctx->device >= 0 && ctx->device < 64) ? (1ull << ctx->device) : 0ull;
+        if (!bit || !(wide.done.load(std::memory_order_acquire) & bit)) {
+            LTCA_CUDA_OK(ctx, cudaFuncSetAttribute(kv8_decode_kernel<T, D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            wide.done.fetch_or(bit, std::memory_order_release);
+        }
+    }
+    LTCA_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kv8_decode_kernel<T, D, NT>, a, k_map, v_map));
     return LTCA_OK;
 }
 template <typename T, int D>
@@ -856,7 +1004,7 @@ int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_dec
     a.nb = (c->S + c->block - 1) / c->block;
     a.G = p->Hq / c->H;
     a.R = a.G * p->Sq;
-    a.tiles = s.tiles; a.rows = s.rows; a.warps = s.warps;
+    a.tiles = s.tiles; a.rows = s.rows; a.warps = s.warps; a.splits = s.splits;
     const int es = elem_size(p->dtype);
     auto on = [&](const void* ptr, const ltca_strides& st, int to) {
         return !((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(st.batch * es) | (uintptr_t)(st.head * es) | (uintptr_t)(st.seq * es)) & (to - 1));
@@ -872,7 +1020,7 @@ int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_dec
                 (c->B > 1 && c->v_strides.batch ? 4 : 0) | (c->H > 1 && c->v_strides.head ? 8 : 0);
     a.status = ctx->d_status;
     const size_t need = partial_bytes(c, s);
-    if (!p->workspace || p->workspace_bytes < need) return fail(ctx, LTCA_ERR_WORKSPACE, "decode needs %zu bytes of workspace", need);
+    if (need && (!p->workspace || p->workspace_bytes < need)) return fail(ctx, LTCA_ERR_WORKSPACE, "decode needs %zu bytes of workspace", need);
     a.partial = reinterpret_cast<float*>(p->workspace);
     return p->dtype == LTCA_BF16 ? launch_width<__nv_bfloat16>(ctx, a, s.nt) : launch_width<float>(ctx, a, s.nt);
 }
