@@ -37,7 +37,7 @@ namespace {
 constexpr int kWarps = 4;                   // of a CTA
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHead = 48;                   // a step's positions and scales
-constexpr int kMaxCluster = 16;             // CTAs that join their shares through shared memory
+constexpr int kMaxCluster = 8;              // CTAs that join their shares through shared memory
 constexpr int kClusterSteps = 8;            // of a warp there, at most
 constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do
 constexpr int kUnitCost = 2;                // what a unit costs beside its steps, in steps
@@ -68,6 +68,7 @@ struct DecodeArgs {
     int strides;                // what has a stride of its own: sequences of k (1) and v (4), heads of k (2) and v (8)
     int splits;                 // CTAs (a cluster) of a unit; 0: the warps share one line
     float* partial;             // [2 warps][rows][D + 4]
+    int2* shares;               // [units]: the warp that has a unit's first step, and how many after it have others
     uint32_t* status;
 };
 
@@ -79,11 +80,11 @@ __device__ __forceinline__ int steps_of(const DecodeArgs& a, int b) {
     if (a.p.blocks) return (a.p.n_blocks * (a.c.block >> 4) + sg - 1) / sg;
     return (live + 16 * sg - 1) / (16 * sg);
 }
-__device__ __forceinline__ int64_t cost_of(const DecodeArgs& a, int b) {                     // of all its units
-    const int steps = steps_of(a, b);
-    return steps == 0 ? 0 : (int64_t)(steps + kUnitCost) * (a.c.H * a.tiles);
-}
-// Warps that get a run of the line; where warp w's begins; whose a place is.
+// A unit's head of keys and tile; a row's new token (rows: new token first, then the heads that share).
+__device__ __forceinline__ int head_of(const DecodeArgs& a, int unit) { return a.tiles == 1 ? unit : unit / a.tiles; }
+__device__ __forceinline__ int tile_of(const DecodeArgs& a, int unit) { return a.tiles == 1 ? 0 : unit % a.tiles; }
+__device__ __forceinline__ int token_of(const DecodeArgs& a, int gr) { return a.p.Sq == 1 ? 0 : gr / a.G; }
+// Warps that get a run of the line; where warp w's begins; whose a place of the line is.
 __device__ __forceinline__ int warps_of(const DecodeArgs& a, int64_t total) {
     return (int)min((int64_t)a.warps, (total + kMinCost - 1) / kMinCost);
 }
@@ -91,7 +92,7 @@ __device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {              
     return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 __device__ __forceinline__ int64_t run_begin(int64_t total, int warps, int w) { return divided(total * w, warps); }
-__device__ __forceinline__ int warp_of(int64_t total, int warps, int64_t at) { return (int)divided((at + 1) * warps - 1, total); }
+__device__ __forceinline__ int warp_at(int64_t total, int warps, int64_t at) { return (int)divided((at + 1) * warps - 1, total); }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -174,10 +175,10 @@ struct Group {
     static __device__ __forceinline__ int k_dim(int c, int w) { return D == 32 ? c * 8 + 4 * w : (w >> 2) * 64 + c * 16 + 4 * (w & 3); }
 };
 
-// The shares of a row joined by a CTA: its warps take shares in turn, a lane D/32 channels of each.  part(k): share k's m, e, l
-// and its sums behind them.
-template <typename T, int D, typename Part>
-__device__ __forceinline__ void join_row(int parts, Part part, float (&sm_o)[kWarps][D], T* out, float* lse) {
+// The shares of a row joined by a CTA whose warps take them in turn (kWide), or by a warp; a lane has D/32 channels.  part(k):
+// share k's m, e, l and its sums behind them.
+template <typename T, int D, bool kWide, typename Part>
+__device__ __forceinline__ void join_row(int parts, Part part, float (*sm_o)[D], T* out, float* lse) {
     constexpr int E = D / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float M = kNone, L = 0.f, top = -INFINITY;
@@ -198,22 +199,37 @@ __device__ __forceinline__ void join_row(int parts, Part part, float (&sm_o)[kWa
 #pragma unroll
     for (int x = 0; x < E; ++x) sum[x] = 0.f;
 #pragma unroll 4
-    for (int k = warp; k < parts; k += kWarps) {
+    for (int k = kWide ? warp : 0; k < parts; k += kWide ? kWarps : 1) {
         const float* src = part(k);
         const float by = exp2_fast((src[0] - M) + src[1] - top);
-#pragma unroll
-        for (int x = 0; x < E; ++x) sum[x] = fmaf(src[4 + lane + 32 * x], by, sum[x]);
+        if constexpr (E == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(src + 4 + lane * 4);
+            sum[0] = fmaf(x.x, by, sum[0]); sum[1] = fmaf(x.y, by, sum[1]); sum[2] = fmaf(x.z, by, sum[2]); sum[3] = fmaf(x.w, by, sum[3]);
+        } else if constexpr (E == 2) {
+            const float2 x = *reinterpret_cast<const float2*>(src + 4 + lane * 2);
+            sum[0] = fmaf(x.x, by, sum[0]); sum[1] = fmaf(x.y, by, sum[1]);
+        } else {
+            sum[0] = fmaf(src[4 + lane], by, sum[0]);
+        }
     }
+    if constexpr (kWide) {
 #pragma unroll
-    for (int x = 0; x < E; ++x) sm_o[warp][lane + 32 * x] = sum[x];
-    __syncthreads();
-    if (tid < D) {
-        float y = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) y += sm_o[w][tid];
-        st_value(out + tid, L == 0.f ? 0.f : y * (pow2((int)top - 6) / L));
+        for (int x = 0; x < E; ++x) sm_o[warp][lane * E + x] = sum[x];
+        __syncthreads();
     }
-    if (tid == 0 && lse) *lse = L == 0.f ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
+    const float by = L == 0.f ? 0.f : pow2((int)top - 6) / L;
+    if constexpr (kWide) {
+        if (tid < D) {
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) y += sm_o[w][tid];
+            st_value(out + tid, L == 0.f ? 0.f : y * by);
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < E; ++x) st_value(out + lane * E + x, L == 0.f ? 0.f : sum[x] * by);
+    }
+    if ((kWide ? tid : lane) == 0 && lse) *lse = L == 0.f ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
 }
 
 template <typename T, int D, int NT>
@@ -230,9 +246,14 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     __shared__ __align__(8) uint64_t sm_bar[kWarps][ST];
     __shared__ int64_t sm_before[kThreads + 1];                   // the line up to each thread's sequences
     __shared__ int64_t sm_warp[kWarps];
+    __shared__ int sm_steps[kThreads];
     __shared__ uint32_t sm_abort;
     __shared__ float sm_join[kWarps][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
+    if (tid == 0) {
+        tma_prefetch_desc(&k_map);
+        tma_prefetch_desc(&v_map);
+    }
     if (lane < ST) mbar_init(smem_u32(&sm_bar[warp][lane]), 1);
     mbar_fence_init();
     if (tid == 0) sm_abort = 0;
@@ -242,7 +263,8 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     // a sequence, a unit of it and a step of that
     struct Cursor { int b, unit, s, steps; };
     Cursor f, end;                                                // what is fetched next; the last step of the run
-    int me = 0;
+    int me = 0, line_warps = 0;
+    int64_t line_total = 0;
     if (a.splits) {
         const int unit = blockIdx.x / a.splits, parts = kWarps * a.splits, w = (blockIdx.x % a.splits) * kWarps + warp;
         f.b = unit / per_b;
@@ -254,7 +276,11 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     } else {
         const int chunk = (a.c.B + kThreads - 1) / kThreads;      // sequences of a thread
         int64_t run = 0;
-        for (int b = tid * chunk; b < min((tid + 1) * chunk, a.c.B); ++b) run += cost_of(a, b);
+        for (int b = tid * chunk; b < min((tid + 1) * chunk, a.c.B); ++b) {
+            const int steps = steps_of(a, b);
+            if (steps) run += (int64_t)(steps + kUnitCost) * per_b;
+            if (chunk == 1) sm_steps[tid] = steps;
+        }
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const int64_t o = __shfl_up_sync(0xffffffffu, run, off);
@@ -270,27 +296,33 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         const int warps = warps_of(a, total);
         me = warp * gridDim.x + blockIdx.x;
         if (me >= warps) return;
-        auto locate = [&](int64_t place) -> Cursor {              // s < 0: in the blank before the steps
-            Cursor x;
-            int i = 0;
+        // the lower lanes look for the run's first place, the upper ones for its last
+        const int64_t place = lane < 16 ? run_begin(total, warps, me) : run_begin(total, warps, me + 1) - 1;
+        int i = 0;
 #pragma unroll
-            for (int y = kThreads / 2; y > 0; y >>= 1)
-                if (sm_before[i + y] <= place) i += y;            // the last thread whose sequences begin at or before it
-            int64_t at = sm_before[i];
-            x.b = i * chunk;
+        for (int y = kThreads / 2; y > 0; y >>= 1)
+            if (sm_before[i + y] <= place) i += y;                // the last thread whose sequences begin at or before it
+        int64_t at = place - sm_before[i];
+        Cursor x;
+        x.b = i * chunk;
+        if (chunk == 1) {
+            x.steps = sm_steps[i];
+        } else {
             for (;; ++x.b) {
-                const int64_t cost = cost_of(a, x.b);
-                if (place - at < cost) break;
-                at += cost;
+                x.steps = steps_of(a, x.b);
+                const int64_t cost = x.steps == 0 ? 0 : (int64_t)(x.steps + kUnitCost) * per_b;
+                if (at < cost) break;
+                at -= cost;
             }
-            x.steps = steps_of(a, x.b);
-            x.unit = (int)divided(place - at, x.steps + kUnitCost);
-            x.s = (int)(place - at - (int64_t)x.unit * (x.steps + kUnitCost)) - kUnitCost;
-            return x;
-        };
-        f = locate(run_begin(total, warps, me));
-        f.s = max(f.s, 0);
-        end = locate(run_begin(total, warps, me + 1) - 1);
+        }
+        x.unit = (int)divided(at, x.steps + kUnitCost);
+        x.s = (int)(at - (int64_t)x.unit * (x.steps + kUnitCost)) - kUnitCost;              // below zero: in the blank
+        f = {__shfl_sync(0xffffffffu, x.b, 0), __shfl_sync(0xffffffffu, x.unit, 0), max(__shfl_sync(0xffffffffu, x.s, 0), 0),
+             __shfl_sync(0xffffffffu, x.steps, 0)};
+        end = {__shfl_sync(0xffffffffu, x.b, 31), __shfl_sync(0xffffffffu, x.unit, 31), __shfl_sync(0xffffffffu, x.s, 31),
+               __shfl_sync(0xffffffffu, x.steps, 31)};
+        line_total = total;
+        line_warps = warps;
     }
     // steps of the run in the unit that x is in
     auto left_of = [&](const Cursor& x) -> int { return (x.b == end.b && x.unit == end.unit ? end.s + 1 : x.steps) - x.s; };
@@ -318,16 +350,16 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     int f_live, f_h;
     int next_blk;                                                 // this lane's entry of the list (lane / 2: a group) for the next fetch
     auto fetch_unit = [&]() {
-        f_h = f.unit / a.tiles;
+        f_h = head_of(a, f.unit);
         const int64_t pair = (int64_t)f.b * a.c.H + f_h;
         sp = (lane & 1 ? a.c.v_scale : a.c.k_scale) + pair * a.nb;
         list = a.p.blocks ? a.p.blocks + pair * a.p.n_blocks : nullptr;
         f_live = a.p.kv_len ? min(a.p.kv_len[f.b], a.c.S) : a.c.S;
         // its queries are needed soon
-        const int gr = (f.unit % a.tiles) * ROWS + lane;
+        const int gr = (tile_of(a, f.unit)) * ROWS + lane;
         if (lane < ROWS && gr < a.R)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const T*>(a.p.q) + f.b * a.p.q_strides.batch +
-                (int64_t)(f_h * a.G + gr % a.G) * a.p.q_strides.head + (int64_t)(gr / a.G) * a.p.q_strides.seq));
+                (int64_t)(f_h * a.G + gr - token_of(a, gr) * a.G) * a.p.q_strides.head + (int64_t)(token_of(a, gr)) * a.p.q_strides.seq));
     };
     auto look_ahead = [&]() {
         const int at = (f.s * SG + min(lane >> 1, SG - 1)) >> log_gpb;
@@ -364,7 +396,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 }
             }
             if (a.p.keep_mask) {
-                const int i0 = (f.unit % a.tiles) * ROWS / a.G, rows = min(a.mask_rows, a.p.Sq - i0);
+                const int i0 = token_of(a, tile_of(a, f.unit) * ROWS), rows = min(a.mask_rows, a.p.Sq - i0);
 #pragma unroll
                 for (int x = 0; x < SG / 2; ++x) {                 // 32 keys at a time
                     const int base = __shfl_sync(0xffffffffu, pos, 4 * x + 2 * (lane >> 4));
@@ -412,11 +444,11 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         }
     };
     auto start_unit = [&]() {
-        const int tile = u.unit % a.tiles, h = u.unit / a.tiles;
+        const int tile = tile_of(a, u.unit), h = head_of(a, u.unit);
         const int n = new_tokens(a.p.new_len, u.b, a.p.Sq);
         const int len = a.p.kv_len ? a.p.kv_len[u.b] : a.c.S, live = min(max(len, 0), a.c.S);
         auto lim_of = [&](int row) -> int {
-            const int gr = tile * ROWS + row, i = gr / a.G;
+            const int gr = tile * ROWS + row, i = token_of(a, gr);
             if (gr >= a.R || i >= n) return 0;
             return a.p.causal ? (int)min((int64_t)live, max((int64_t)len - n + i + 1, (int64_t)0)) : live;
         };
@@ -425,9 +457,9 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int gr = tile * ROWS + t * 8 + r;
-            const bool there = gr < a.R && gr / a.G < n;
+            const bool there = gr < a.R && token_of(a, gr) < n;
             const T* q = reinterpret_cast<const T*>(a.p.q) + u.b * a.p.q_strides.batch +
-                         (int64_t)(h * a.G + gr % a.G) * a.p.q_strides.head + (int64_t)(gr / a.G) * a.p.q_strides.seq;
+                         (int64_t)(h * a.G + gr - token_of(a, gr) * a.G) * a.p.q_strides.head + (int64_t)(token_of(a, gr)) * a.p.q_strides.seq;
             float x[W][4];
             uint32_t most = 0;
 #pragma unroll
@@ -474,8 +506,8 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) mask_row |= (uint64_t)(min((tile0 + t * 8 + 2 * c + k) / a.G - tile0 / a.G, 31)) << (8 * (2 * t + k));
-            mask_rows = min(a.mask_rows, a.p.Sq - tile0 / a.G);
+                for (int k = 0; k < 2; ++k) mask_row |= (uint64_t)(min(token_of(a, tile0 + t * 8 + 2 * c + k) - token_of(a, tile0), 31)) << (8 * (2 * t + k));
+            mask_rows = min(a.mask_rows, a.p.Sq - token_of(a, tile0));
         }
         if constexpr (!kQRegs) __syncwarp();
     };
@@ -740,7 +772,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 
     // ---- a unit's sums leave: finished where this warp has seen all of it, else to scratch ----
     auto end_unit = [&](bool mine, float* slot) {
-        const int tile = u.unit % a.tiles, h = u.unit / a.tiles;
+        const int tile = tile_of(a, u.unit), h = head_of(a, u.unit);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -753,8 +785,8 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 if (mine) {
                     const bool dead = lim[t][x] == 0 || sum == 0.f;
                     const float by = pow2((int)e[t][x] - 6) / sum;
-                    T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
-                             (int64_t)(gr / a.G) * a.p.o_strides.seq + r * (D / 8);
+                    T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - token_of(a, gr) * a.G) * a.p.o_strides.head +
+                             (int64_t)(token_of(a, gr)) * a.p.o_strides.seq + r * (D / 8);
 #pragma unroll
                     for (int i = 0; i < W; i += 2) {
                         const float y[4] = {dead ? 0.f : o[t][i][x] * by, dead ? 0.f : o[t][i][x + 2] * by,
@@ -762,7 +794,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                         store4(out + 2 * i, a.vec_o != 0, y);
                     }
                     if (r == 0 && a.p.lse)
-                        a.p.lse[((int64_t)u.b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + gr / a.G] =
+                        a.p.lse[((int64_t)u.b * a.p.Hq + h * a.G + gr - token_of(a, gr) * a.G) * a.p.Sq + token_of(a, gr)] =
                             dead ? -INFINITY : (m[t][x] == kNone ? 0.f : m[t][x] * 0.693147181f) + logf(sum);
                 } else {
                     float* dst = slot + row * (D + 4);
@@ -797,6 +829,11 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         ++u.s;
         if (--u_left > 0 || a.splits) continue;
         const bool to_end = u.s == u.steps;
+        if (from_start && lane == 0) {
+            // the run ends in this unit, whose last step is as many places on as it has steps left
+            const int64_t last = run_begin(line_total, line_warps, me + 1) - 1 + (u.steps - u.s);
+            a.shares[(int64_t)u.b * per_b + u.unit] = make_int2(me, to_end ? 0 : warp_at(line_total, line_warps, last) - me);
+        }
         end_unit(from_start && to_end, a.partial + (int64_t)(2 * me + (to_end ? 0 : from_start ? 1 : 0)) * a.rows * (D + 4));
         if (at_end(u)) break;
         next_unit(u);
@@ -806,6 +843,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         start_unit();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    grid_launch_dependents();                                     // the join's CTAs may come as these leave
     if (!a.splits) return;
 
     // ---- the cluster's shares, over the rings; its CTAs take the rows in turn ----
@@ -816,19 +854,19 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     end_unit(false, share + warp * a.rows * (D + 4));
     if (a.splits > 1) cluster.sync();
     else __syncthreads();
-    const int tile = u.unit % a.tiles, h = u.unit / a.tiles, rank = blockIdx.x % a.splits;
+    const int tile = tile_of(a, u.unit), h = head_of(a, u.unit), rank = blockIdx.x % a.splits;
     const int n = new_tokens(a.p.new_len, u.b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[u.b] : a.c.S;
     for (int row = rank; row < ROWS && tile * ROWS + row < a.R; row += a.splits) {
-        const int gr = tile * ROWS + row, i = gr / a.G;
-        T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
+        const int gr = tile * ROWS + row, i = token_of(a, gr);
+        T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - token_of(a, gr) * a.G) * a.p.o_strides.head +
                  (int64_t)i * a.p.o_strides.seq;
-        float* lse = a.p.lse ? a.p.lse + ((int64_t)u.b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + i : nullptr;
+        float* lse = a.p.lse ? a.p.lse + ((int64_t)u.b * a.p.Hq + h * a.G + gr - token_of(a, gr) * a.G) * a.p.Sq + i : nullptr;
         if (len <= 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
             if (tid < D) st_value(out + tid, 0.f);
             if (tid == 0 && lse) *lse = -INFINITY;
             continue;
         }
-        join_row<T, D>(kWarps * a.splits, [&](int k) -> const float* {
+        join_row<T, D, true>(kWarps * a.splits, [&](int k) -> const float* {
             const float* mine = share + ((k & (kWarps - 1)) * a.rows + row) * (D + 4);
             return a.splits > 1 ? cluster.map_shared_rank(mine, k / kWarps) : mine;
         }, sm_join, out, lse);
@@ -837,50 +875,33 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     if (a.splits > 1) cluster.sync();                               // until nobody reads this CTA's shared memory
 }
 
-// The warps' shares of a unit's row joined; what no warp or a single one has seen is zeros, or finished already.  One CTA per
-// row: its warps take shares in turn, a lane D/32 channels of each.
-template <typename T, int D>
+// The warps' shares of a unit's rows joined; what no warp or a single one has seen is zeros, or finished already.  kWide: a CTA
+// per row, for many shares; else a warp.
+template <typename T, int D, bool kWide>
 __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_constant__ DecodeArgs a, int tile_rows) {
-    __shared__ int64_t sm_sum[2][kWarps];
-    __shared__ float sm_o[kWarps][D];
+    __shared__ float sm_o[kWide ? kWarps : 1][D];
     grid_dependency_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int unit = (int)(blockIdx.x % (unsigned)(a.c.H * a.tiles)), b = (int)(blockIdx.x / (unsigned)(a.c.H * a.tiles));
-    const int tile = unit % a.tiles, h = unit / a.tiles, row = blockIdx.y, gr = tile * tile_rows + row;
-    if (gr >= a.R) return;
-    int64_t before = 0, total = 0;
-    for (int x = tid; x < a.c.B; x += kThreads) {
-        const int64_t s = cost_of(a, x);
-        total += s;
-        if (x < b) before += s;
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, off);
-        before += __shfl_xor_sync(0xffffffffu, before, off);
-    }
-    if (lane == 0) { sm_sum[0][warp] = total; sm_sum[1][warp] = before; }
-    __syncthreads();
-    total = before = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) { total += sm_sum[0][w]; before += sm_sum[1][w]; }
-    const int steps = steps_of(a, b), i = gr / a.G;
-    T* out = reinterpret_cast<T*>(a.p.o) + b * a.p.o_strides.batch + (int64_t)(h * a.G + gr % a.G) * a.p.o_strides.head +
+    const int per_b = a.c.H * a.tiles, unit = (int)(blockIdx.x % (unsigned)per_b), b = (int)(blockIdx.x / (unsigned)per_b);
+    const int tile = tile_of(a, unit), h = head_of(a, unit), row = kWide ? blockIdx.y : blockIdx.y * kWarps + warp;
+    const int gr = tile * tile_rows + row;
+    if (row >= a.rows || gr >= a.R) return;
+    const int2 who = a.shares[blockIdx.x];
+    const int steps = steps_of(a, b), i = token_of(a, gr);
+    T* out = reinterpret_cast<T*>(a.p.o) + b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - i * a.G) * a.p.o_strides.head +
              (int64_t)i * a.p.o_strides.seq;
-    float* lse = a.p.lse ? a.p.lse + ((int64_t)b * a.p.Hq + h * a.G + gr % a.G) * a.p.Sq + i : nullptr;
+    float* lse = a.p.lse ? a.p.lse + ((int64_t)b * a.p.Hq + h * a.G + gr - i * a.G) * a.p.Sq + i : nullptr;
     const int n = new_tokens(a.p.new_len, b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[b] : a.c.S;
+    const int first = kWide ? tid : lane;
     if (steps == 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
-        if (tid < D) st_value(out + tid, 0.f);
-        if (tid == 0 && lse) *lse = -INFINITY;
+        for (int d = first; d < D; d += kWide ? kThreads : 32) st_value(out + d, 0.f);
+        if (first == 0 && lse) *lse = -INFINITY;
         return;
     }
-    const int64_t s0 = before + (int64_t)unit * (steps + kUnitCost) + kUnitCost;       // its first step's place
-    const int warps = warps_of(a, total), w0 = warp_of(total, warps, s0), w1 = warp_of(total, warps, s0 + steps - 1);
-    if (w0 == w1) return;
-    const int parts = w1 - w0 + 1;
+    if (who.y == 0) return;
     // the first share is the last thing that its warp did, the others the first
-    auto part = [&](int k) { return a.partial + ((int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * a.rows + row) * (D + 4); };
-    join_row<T, D>(parts, part, sm_o, out, lse);
+    auto part = [&](int k) -> const float* { return a.partial + ((int64_t)(2 * (who.x + k) + (k == 0 ? 1 : 0)) * a.rows + row) * (D + 4); };
+    join_row<T, D, kWide>(who.y + 1, part, sm_o, out, lse);
 }
 
 // How a call is cut up; a function of the problem alone, so that the size query and the launch agree.
@@ -916,6 +937,9 @@ Plan plan_of(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
 size_t partial_bytes(const ltca_kv8_cache* c, const Plan& s) {
     return align_up((size_t)2 * s.warps * s.rows * (c->D + 4) * sizeof(float), 256);
 }
+size_t shares_bytes(const ltca_kv8_cache* c, const Plan& s) {
+    return s.splits ? 0 : align_up((size_t)c->B * c->H * s.tiles * sizeof(int2), 256);
+}
 
 // Keys or values as TMA sees them: [B, H, S, D] bytes, `box` keys a copy.
 int make_map(ltca_ctx* ctx, CUtensorMap* map, const void* base, const ltca_strides& st, const DecodeArgs& a, int own) {
@@ -949,7 +973,11 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
     if (!a.splits) {
         const dim3 grid((unsigned)((a.warps + kWarps - 1) / kWarps));
         LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_kernel<T, D, NT>, grid, dim3(kThreads), bytes, ctx->stream, a, k_map, v_map));
-        LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_join_kernel<T, D>, dim3((unsigned)units, (unsigned)a.rows), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
+        // a CTA for each row where a unit has many shares
+        const bool wide = a.warps > 16 * units;
+        auto join = wide ? kv8_decode_join_kernel<T, D, true> : kv8_decode_join_kernel<T, D, false>;
+        const dim3 rows((unsigned)units, (unsigned)(wide ? a.rows : (a.rows + kWarps - 1) / kWarps));
+        LTCA_CUDA_OK(ctx, launch_dependent(join, dim3(rows), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
         return LTCA_OK;
     }
     cudaLaunchConfig_t cfg;
@@ -991,7 +1019,10 @@ int launch_width(ltca_ctx* ctx, const DecodeArgs& a, int nt) {
 
 }  // namespace
 
-size_t kv8_decode_workspace(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) { return partial_bytes(c, plan_of(c, p)); }
+size_t kv8_decode_workspace(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
+    const Plan s = plan_of(c, p);
+    return partial_bytes(c, s) + shares_bytes(c, s);
+}
 
 int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     const Plan s = plan_of(c, p);
@@ -1019,9 +1050,10 @@ int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_dec
     a.strides = (c->B > 1 && c->k_strides.batch ? 1 : 0) | (c->H > 1 && c->k_strides.head ? 2 : 0) |
                 (c->B > 1 && c->v_strides.batch ? 4 : 0) | (c->H > 1 && c->v_strides.head ? 8 : 0);
     a.status = ctx->d_status;
-    const size_t need = partial_bytes(c, s);
+    const size_t need = partial_bytes(c, s) + shares_bytes(c, s);
     if (need && (!p->workspace || p->workspace_bytes < need)) return fail(ctx, LTCA_ERR_WORKSPACE, "decode needs %zu bytes of workspace", need);
     a.partial = reinterpret_cast<float*>(p->workspace);
+    a.shares = reinterpret_cast<int2*>(static_cast<char*>(p->workspace) + partial_bytes(c, s));
     return p->dtype == LTCA_BF16 ? launch_width<__nv_bfloat16>(ctx, a, s.nt) : launch_width<float>(ctx, a, s.nt);
 }
 
