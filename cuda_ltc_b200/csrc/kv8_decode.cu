@@ -49,12 +49,14 @@ constexpr float kLimit = 16384.f;           // largest weight before the referen
 constexpr int step_groups(int D) { return D == 32 ? 4 : 2; }
 template <int D> constexpr int kGroups = step_groups(D);
 template <int D> constexpr int kStepBytes = kGroups<D> * 32 * D;
-template <int D> constexpr int kStages = D == 128 ? 2 : 4;
+template <int D> constexpr int kStages = D == 128 ? 2 : 3;
 // CTAs of an SM, by the registers that NT tiles of 8 rows take
-constexpr int ctas_per_sm(int D, int nt) { return nt == 4 || nt * D >= 256 ? 2 : 3; }
+constexpr int ctas_per_sm(int D, int nt) { return nt == 4 || nt * D >= 256 ? 2 : nt == 1 && D <= 64 ? 4 : 3; }
 template <int D, int NT> constexpr int kCtas = ctas_per_sm(D, NT);
-// Tiles of 8 rows that a warp keeps at most: fp32's two terms of 128 channels leave room for two.
-constexpr int most_tiles(int es, int D) { return es == 4 && D == 128 ? 2 : 4; }
+// Tiles of 8 rows that a warp keeps at most: a stage of the ring has room for the rows of Q, and fp32's two terms of 128 channels
+// leave registers for two.
+constexpr int most_tiles(int es, int D) { return es == 4 && D >= 64 ? 2 : 4; }
+constexpr int kLens = 256;                  // lengths in shared memory
 
 struct DecodeArgs {
     ltca_kv8_cache c;
@@ -62,7 +64,7 @@ struct DecodeArgs {
     int nb, G, R;               // blocks of tokens; heads of queries per head of keys; rows of a pair
     int tiles, rows;            // of a pair: tiles of 8 NT rows; rows of a tile that exist (of the first one)
     int warps;                  // that share the line of steps
-    int vec_q, vec_o;           // rows of q start on boundaries of four values, rows of o on 16 bytes
+    int vec_q, vec_o;           // rows of q start on 16-byte boundaries, rows of o on boundaries of four values
     int mask_rows;              // rows of keep_mask that a tile's rows need
     int box;                    // keys of a copy
     int strides;                // what has a stride of its own: sequences of k (1) and v (4), heads of k (2) and v (8)
@@ -73,13 +75,14 @@ struct DecodeArgs {
 };
 
 // Steps of each unit of sequence b.
-__device__ __forceinline__ int steps_of(const DecodeArgs& a, int b) {
-    const int len = a.p.kv_len ? a.p.kv_len[b] : a.c.S, live = min(max(len, 0), a.c.S);
+__device__ __forceinline__ int steps_for(const DecodeArgs& a, int len) {
+    const int live = min(max(len, 0), a.c.S);
     if (live == 0) return 0;
     const int sg = step_groups(a.c.D);
     if (a.p.blocks) return (a.p.n_blocks * (a.c.block >> 4) + sg - 1) / sg;
     return (live + 16 * sg - 1) / (16 * sg);
 }
+__device__ __forceinline__ int length_of(const DecodeArgs& a, int b) { return a.p.kv_len ? a.p.kv_len[b] : a.c.S; }
 // A unit's head of keys and tile; a row's new token (rows: new token first, then the heads that share).
 __device__ __forceinline__ int head_of(const DecodeArgs& a, int unit) { return a.tiles == 1 ? unit : unit / a.tiles; }
 __device__ __forceinline__ int tile_of(const DecodeArgs& a, int unit) { return a.tiles == 1 ? 0 : unit % a.tiles; }
@@ -123,25 +126,29 @@ __device__ __forceinline__ void fetch(uint32_t dst, const void* src) {
     if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
-__device__ __forceinline__ void load4(const float* p, bool vec, float (&x)[4]) {
-    if (vec) {
-        const float4 u = __ldg(reinterpret_cast<const float4*>(p));
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = p[i];
+// Four channels of a row of Q as they lie in memory: the largest magnitude so far (an infinity or NaN shows as 2^128 or more),
+// the largest finite one, and the values.
+struct Four32 {
+    float4 v;
+    __device__ __forceinline__ void largest(uint32_t& m) const {
+        m = max(max(m, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu,
+            max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
     }
-}
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, bool vec, float (&x)[4]) {
-    if (vec) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-        x[0] = __uint_as_float(u.x << 16); x[1] = __uint_as_float(u.x & 0xffff0000u);
-        x[2] = __uint_as_float(u.y << 16); x[3] = __uint_as_float(u.y & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+    __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+};
+struct Four16 {
+    uint2 v;
+    __device__ __forceinline__ void largest(uint32_t& m) const {
+        const uint32_t t = __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+        m = max(m, max(t << 16, t & 0xffff0000u));
     }
-}
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+};
+template <typename T> struct FourOf { using type = Four32; };
+template <> struct FourOf<__nv_bfloat16> { using type = Four16; };
 __device__ __forceinline__ void store4(float* p, bool vec, const float (&x)[4]) {
     if (vec) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
     else
@@ -246,7 +253,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     __shared__ __align__(8) uint64_t sm_bar[kWarps][ST];
     __shared__ int64_t sm_before[kThreads + 1];                   // the line up to each thread's sequences
     __shared__ int64_t sm_warp[kWarps];
-    __shared__ int sm_steps[kThreads];
+    __shared__ int sm_len[kLens];
     __shared__ uint32_t sm_abort;
     __shared__ float sm_join[kWarps][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
@@ -260,6 +267,9 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     grid_dependency_wait();
 
     const int per_b = a.c.H * a.tiles;                            // units of a sequence
+    // (from shared memory where they are there: a load takes microseconds while the ring's copies have the way to the SM)
+    auto len_of = [&](int b) -> int { return !a.splits && b < kLens ? sm_len[b] : length_of(a, b); };
+    auto steps_of = [&](int b) -> int { return steps_for(a, len_of(b)); };
     // a sequence, a unit of it and a step of that
     struct Cursor { int b, unit, s, steps; };
     Cursor f, end;                                                // what is fetched next; the last step of the run
@@ -269,7 +279,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         const int unit = blockIdx.x / a.splits, parts = kWarps * a.splits, w = (blockIdx.x % a.splits) * kWarps + warp;
         f.b = unit / per_b;
         f.unit = unit % per_b;
-        f.steps = steps_of(a, f.b);
+        f.steps = steps_of(f.b);
         end = f;
         f.s = (int)((uint32_t)f.steps * w / parts);
         end.s = (int)((uint32_t)f.steps * (w + 1) / parts) - 1;
@@ -277,9 +287,9 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         const int chunk = (a.c.B + kThreads - 1) / kThreads;      // sequences of a thread
         int64_t run = 0;
         for (int b = tid * chunk; b < min((tid + 1) * chunk, a.c.B); ++b) {
-            const int steps = steps_of(a, b);
+            const int len = length_of(a, b), steps = steps_for(a, len);
             if (steps) run += (int64_t)(steps + kUnitCost) * per_b;
-            if (chunk == 1) sm_steps[tid] = steps;
+            if (b < kLens) sm_len[b] = len;
         }
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -305,15 +315,11 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         int64_t at = place - sm_before[i];
         Cursor x;
         x.b = i * chunk;
-        if (chunk == 1) {
-            x.steps = sm_steps[i];
-        } else {
-            for (;; ++x.b) {
-                x.steps = steps_of(a, x.b);
-                const int64_t cost = x.steps == 0 ? 0 : (int64_t)(x.steps + kUnitCost) * per_b;
-                if (at < cost) break;
-                at -= cost;
-            }
+        for (;; ++x.b) {
+            x.steps = steps_of(x.b);
+            const int64_t cost = x.steps == 0 ? 0 : (int64_t)(x.steps + kUnitCost) * per_b;
+            if (at < cost) break;
+            at -= cost;
         }
         x.unit = (int)divided(at, x.steps + kUnitCost);
         x.s = (int)(at - (int64_t)x.unit * (x.steps + kUnitCost)) - kUnitCost;              // below zero: in the blank
@@ -333,7 +339,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         x.s = 0;
         if (++x.unit == per_b) {
             x.unit = 0;
-            do x.steps = steps_of(a, ++x.b); while (x.steps == 0);
+            do x.steps = steps_of(++x.b); while (x.steps == 0);
         }
     };
     auto at_end = [&](const Cursor& x) { return x.b == end.b && x.unit == end.unit; };
@@ -348,33 +354,69 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     const float* sp;                                              // of the fetched unit: k's scales for even lanes, v's for odd ones
     const int32_t* list;
     int f_live, f_h;
-    int next_blk;                                                 // this lane's entry of the list (lane / 2: a group) for the next fetch
+    bool f_q = true;                                              // the unit's queries come first, in a stage of their own
+    int win, win_next, win_at;                                    // 32 entries of the list, a lane each, the next 32, and where they are
+    auto list_at = [&](int i) -> int { return i < a.p.n_blocks ? list[i] : -1; };
     auto fetch_unit = [&]() {
         f_h = head_of(a, f.unit);
         const int64_t pair = (int64_t)f.b * a.c.H + f_h;
         sp = (lane & 1 ? a.c.v_scale : a.c.k_scale) + pair * a.nb;
         list = a.p.blocks ? a.p.blocks + pair * a.p.n_blocks : nullptr;
-        f_live = a.p.kv_len ? min(a.p.kv_len[f.b], a.c.S) : a.c.S;
-        // its queries are needed soon
-        const int gr = (tile_of(a, f.unit)) * ROWS + lane;
-        if (lane < ROWS && gr < a.R)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const T*>(a.p.q) + f.b * a.p.q_strides.batch +
-                (int64_t)(f_h * a.G + gr - token_of(a, gr) * a.G) * a.p.q_strides.head + (int64_t)(token_of(a, gr)) * a.p.q_strides.seq));
+        f_live = min(len_of(f.b), a.c.S);
+        f_q = true;
+        if (list) {
+            win_at = (f.s * SG >> log_gpb) & ~31;
+            win = list_at(win_at + lane);
+            win_next = list_at(win_at + 32 + lane);
+        }
     };
-    auto look_ahead = [&]() {
-        const int at = (f.s * SG + min(lane >> 1, SG - 1)) >> log_gpb;
-        next_blk = at < a.p.n_blocks ? list[at] : -1;
+    auto fetch_queries = [&](uint32_t body, uint32_t bar) {
+        // lane: a row's place
+        const int mine = tile_of(a, f.unit) * ROWS + lane, token = token_of(a, mine);
+        const int64_t place = f.b * a.p.q_strides.batch + (int64_t)(f_h * a.G + mine - token * a.G) * a.p.q_strides.head +
+                              (int64_t)token * a.p.q_strides.seq;
+        const int rows = min(ROWS, a.R - tile_of(a, f.unit) * ROWS);
+        const T* q = reinterpret_cast<const T*>(a.p.q);
+        if (a.vec_q) {
+            constexpr int kChunks = D * (int)sizeof(T) / 16;      // of a row
+#pragma unroll
+            for (int j = 0; j < ROWS * kChunks / 32; ++j) {
+                const int row = (j * 32 + lane) / kChunks, chunk = (j * 32 + lane) % kChunks;
+                const T* src = q + __shfl_sync(0xffffffffu, place, row) + chunk * (16 / (int)sizeof(T));
+                if (row < rows) fetch<16>(body + (j * 32 + lane) * 16, src);
+            }
+        } else {                                                  // rows that start on any element
+            T* dst = reinterpret_cast<T*>(smem + (body - smem_u32(smem)));
+            for (int row = 0; row < rows; ++row) {
+                const T* src = q + __shfl_sync(0xffffffffu, place, row);
+#pragma unroll
+                for (int d = 0; d < D; d += 32) dst[row * D + d + lane] = src[d + lane];
+            }
+        }
+        if (lane == 0) mbar_arrive(bar);
     };
     auto fetch_step = [&](int stage) {
-        if (f_left > 0) {
+        if (f_left > 0 && f_q) {
+            fetch_queries(smem_u32(ring + stage * kStepBytes<D>), smem_u32(&sm_bar[warp][stage]));
+            f_q = false;
+        } else if (f_left > 0) {
             const uint32_t head = smem_u32(heads + stage * extra), body = smem_u32(ring + stage * kStepBytes<D>);
             const uint32_t bar = smem_u32(&sm_bar[warp][stage]);
             // lanes 2g and 2g + 1: where group g is
-            int pos = kNowhere;
+            int pos = kNowhere, blk = -1;
+            if (list) {
+                const int e = (f.s * SG + min(lane >> 1, SG - 1)) >> log_gpb;
+                if (__shfl_sync(0xffffffffu, e, 0) >= win_at + 32) {
+                    win_at += 32;
+                    win = win_next;
+                    win_next = list_at(win_at + 32 + lane);
+                }
+                blk = __shfl_sync(0xffffffffu, win, e - win_at);
+            }
             if (lane < 2 * SG) {
                 const int g = f.s * SG + (lane >> 1);
                 if (!list) pos = g << 4;
-                else if (next_blk >= 0 && next_blk < a.nb) pos = (next_blk << log_block) + ((g & ((1 << log_gpb) - 1)) << 4);
+                else if (blk >= 0 && blk < a.nb) pos = (blk << log_block) + ((g & ((1 << log_gpb) - 1)) << 4);
                 if (pos >= f_live) pos = kNowhere;
                 asm volatile("st.shared.b32 [%0], %1;" ::"r"(head + (lane >> 1) * 4), "r"(pos) : "memory");
                 if (pos != kNowhere) fetch<4>(head + 16 + lane * 4, sp + (pos >> log_block));
@@ -413,14 +455,10 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 f_left = left_of(f);
                 if (f_left > 0) fetch_unit();
             }
-            if (list && f_left > 0) look_ahead();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (f_left > 0) {
-        fetch_unit();
-        if (list) look_ahead();
-    }
+    if (f_left > 0) fetch_unit();
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) fetch_step(i);
 
@@ -443,34 +481,46 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 for (int k = 0; k < 4; ++k) o[t][i][k] = 0.f;
         }
     };
-    auto start_unit = [&]() {
-        const int tile = tile_of(a, u.unit), h = head_of(a, u.unit);
-        const int n = new_tokens(a.p.new_len, u.b, a.p.Sq);
-        const int len = a.p.kv_len ? a.p.kv_len[u.b] : a.c.S, live = min(max(len, 0), a.c.S);
-        auto lim_of = [&](int row) -> int {
-            const int gr = tile * ROWS + row, i = token_of(a, gr);
-            if (gr >= a.R || i >= n) return 0;
-            return a.p.causal ? (int)min((int64_t)live, max((int64_t)len - n + i + 1, (int64_t)0)) : live;
-        };
-        lim_min = 0x7fffffff;
+    auto start_unit = [&](const unsigned char* rows_q) {
+        const int tile = tile_of(a, u.unit), n = new_tokens(a.p.new_len, u.b, a.p.Sq);
+        const int len = len_of(u.b), live = min(max(len, 0), a.c.S);
+        // lane: a row
+        const int mine = tile * ROWS + lane, token = token_of(a, mine);
+        int my_lim = 0;
+        if (lane < ROWS && mine < a.R && token < n)
+            my_lim = a.p.causal ? (int)min((int64_t)live, max((int64_t)len - n + token + 1, (int64_t)0)) : live;
+        lim_min = __reduce_min_sync(0xffffffffu, my_lim > 0 ? my_lim : 0x7fffffff);
+        if (a.p.keep_mask) {
+            const int first = __shfl_sync(0xffffffffu, token, 0), at = min(token - first, 31);
+            mask_row = 0;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) mask_row |= (uint64_t)__shfl_sync(0xffffffffu, at, t * 8 + 2 * c + k) << (8 * (2 * t + k));
+            mask_rows = min(a.mask_rows, a.p.Sq - first);
+        }
         if constexpr (!kQRegs) __syncwarp();
+        using Four = typename FourOf<T>::type;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int gr = tile * ROWS + t * 8 + r;
-            const bool there = gr < a.R && token_of(a, gr) < n;
-            const T* q = reinterpret_cast<const T*>(a.p.q) + u.b * a.p.q_strides.batch +
-                         (int64_t)(h * a.G + gr - token_of(a, gr) * a.G) * a.p.q_strides.head + (int64_t)(token_of(a, gr)) * a.p.q_strides.seq;
-            float x[W][4];
+            const bool there = __shfl_sync(0xffffffffu, my_lim, t * 8 + r) > 0;
+            Four x[W];
             uint32_t most = 0;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                if (there) load4(q + Gr::k_dim(c, w), a.vec_q != 0, x[w]);
-                else x[w][0] = x[w][1] = x[w][2] = x[w][3] = 0.f;
+                x[w] = *reinterpret_cast<const Four*>(reinterpret_cast<const T*>(rows_q) + (t * 8 + r) * D + Gr::k_dim(c, w));
+                x[w].largest(most);
             }
+            if (__any_sync(0xffffffffu, there && most >= 0x7f800000u)) {             // infinities and NaN do not count
+                most = 0;
 #pragma unroll
-            for (int w = 0; w < W; ++w)
+                for (int w = 0; w < W; ++w) {
+                    float y[4];
+                    x[w].get(y);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) most = max(most, finite_abs_bits(x[w][y]));
+                    for (int k = 0; k < 4; ++k) most = max(most, finite_abs_bits(y[k]));
+                }
+            }
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const int ex = min(max((int)(most >> 23) - 127, -100), 120);
@@ -478,15 +528,18 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 float y[4];
+                x[w].get(y);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] = x[w][k] * down;
+                for (int k = 0; k < 4; ++k) y[k] *= down;
                 uint2 hi = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
+                if (!there) hi = make_uint2(0, 0);
                 if constexpr (kQRegs) qf[t][0][w] = hi;
                 else sm_q[warp][t][0][w][lane] = hi;
                 if constexpr (kTerms == 2) {
                     const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
                     const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
                     hi = make_uint2(half2_bits(y[0] - f0.x, y[1] - f0.y), half2_bits(y[2] - f1.x, y[3] - f1.y));
+                    if (!there) hi = make_uint2(0, 0);
                     if constexpr (kQRegs) qf[t][kTerms - 1][w] = hi;
                     else sm_q[warp][t][kTerms - 1][w][lane] = hi;
                 }
@@ -494,21 +547,10 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 cs[t][k] = __shfl_sync(0xffffffffu, up, (2 * c + k) * 4);
-                lim[t][k] = lim_of(t * 8 + 2 * c + k);
-                if (lim[t][k] > 0) lim_min = min(lim_min, lim[t][k]);
+                lim[t][k] = __shfl_sync(0xffffffffu, my_lim, t * 8 + 2 * c + k);
             }
         }
         clear();
-        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
-        if (a.p.keep_mask) {
-            const int tile0 = tile * ROWS;
-            mask_row = 0;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) mask_row |= (uint64_t)(min(token_of(a, tile0 + t * 8 + 2 * c + k) - token_of(a, tile0), 31)) << (8 * (2 * t + k));
-            mask_rows = min(a.mask_rows, a.p.Sq - token_of(a, tile0));
-        }
         if constexpr (!kQRegs) __syncwarp();
     };
     auto q_at = [&](int t, int x, int w) -> uint2 {
@@ -772,7 +814,11 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 
     // ---- a unit's sums leave: finished where this warp has seen all of it, else to scratch ----
     auto end_unit = [&](bool mine, float* slot) {
-        const int tile = tile_of(a, u.unit), h = head_of(a, u.unit);
+        // lane: a row's place
+        const int h = head_of(a, u.unit), my_row = tile_of(a, u.unit) * ROWS + lane, token = token_of(a, my_row);
+        const int head = h * a.G + my_row - token * a.G, rows = min(ROWS, a.R - tile_of(a, u.unit) * ROWS);
+        const int64_t place = u.b * a.p.o_strides.batch + head * a.p.o_strides.head + token * a.p.o_strides.seq;
+        const int64_t lse_place = ((int64_t)u.b * a.p.Hq + head) * a.p.Sq + token;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -780,23 +826,22 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 float sum = l[t][x];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                const int row = t * 8 + 2 * c + x, gr = tile * ROWS + row;
-                if (gr >= a.R) continue;
+                const int row = t * 8 + 2 * c + x;
                 if (mine) {
+                    T* out = reinterpret_cast<T*>(a.p.o) + __shfl_sync(0xffffffffu, place, row) + r * (D / 8);
+                    const int64_t at = __shfl_sync(0xffffffffu, lse_place, row);
                     const bool dead = lim[t][x] == 0 || sum == 0.f;
                     const float by = pow2((int)e[t][x] - 6) / sum;
-                    T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - token_of(a, gr) * a.G) * a.p.o_strides.head +
-                             (int64_t)(token_of(a, gr)) * a.p.o_strides.seq + r * (D / 8);
+                    if (row < rows) {
 #pragma unroll
-                    for (int i = 0; i < W; i += 2) {
-                        const float y[4] = {dead ? 0.f : o[t][i][x] * by, dead ? 0.f : o[t][i][x + 2] * by,
-                                            dead ? 0.f : o[t][i + 1][x] * by, dead ? 0.f : o[t][i + 1][x + 2] * by};
-                        store4(out + 2 * i, a.vec_o != 0, y);
+                        for (int i = 0; i < W; i += 2) {
+                            const float y[4] = {dead ? 0.f : o[t][i][x] * by, dead ? 0.f : o[t][i][x + 2] * by,
+                                                dead ? 0.f : o[t][i + 1][x] * by, dead ? 0.f : o[t][i + 1][x + 2] * by};
+                            store4(out + 2 * i, a.vec_o != 0, y);
+                        }
+                        if (r == 0 && a.p.lse) a.p.lse[at] = dead ? -INFINITY : (m[t][x] == kNone ? 0.f : m[t][x] * 0.693147181f) + logf(sum);
                     }
-                    if (r == 0 && a.p.lse)
-                        a.p.lse[((int64_t)u.b * a.p.Hq + h * a.G + gr - token_of(a, gr) * a.G) * a.p.Sq + token_of(a, gr)] =
-                            dead ? -INFINITY : (m[t][x] == kNone ? 0.f : m[t][x] * 0.693147181f) + logf(sum);
-                } else {
+                } else if (row < rows) {
                     float* dst = slot + row * (D + 4);
                     if (r == 0) *reinterpret_cast<float4*>(dst) = make_float4(m[t][x], e[t][x], sum, 0.f);
 #pragma unroll
@@ -809,9 +854,8 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 
     int stage = 0;
     uint32_t parity = 0;
-    bool from_start = u.s == 0;
-    if (u_left > 0) start_unit();
-    else clear();
+    bool from_start = u.s == 0, u_q = true;
+    if (u_left <= 0) clear();
     while (u_left > 0) {
         fetch_step(stage == 0 ? ST - 1 : stage - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
@@ -822,10 +866,19 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
             break;
         }
         __syncwarp();                                               // the step's head and mask are read by all lanes
+        if (u_q) {
+            start_unit(ring + stage * kStepBytes<D>);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA writes next where these rows lay
+        } else {
 #pragma unroll
-        for (int g = 0; g < SG; g += NG) step(stage, g);
+            for (int g = 0; g < SG; g += NG) step(stage, g);
+        }
         __syncwarp();
         if (++stage == ST) { stage = 0; parity ^= 1; }
+        if (u_q) {
+            u_q = false;
+            continue;
+        }
         ++u.s;
         if (--u_left > 0 || a.splits) continue;
         const bool to_end = u.s == u.steps;
@@ -839,8 +892,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         next_unit(u);
         u_left = left_of(u);
         if (u_left <= 0) break;
-        from_start = true;
-        start_unit();
+        from_start = u_q = true;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     grid_launch_dependents();                                     // the join's CTAs may come as these leave
@@ -855,7 +907,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     if (a.splits > 1) cluster.sync();
     else __syncthreads();
     const int tile = tile_of(a, u.unit), h = head_of(a, u.unit), rank = blockIdx.x % a.splits;
-    const int n = new_tokens(a.p.new_len, u.b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[u.b] : a.c.S;
+    const int n = new_tokens(a.p.new_len, u.b, a.p.Sq), len = length_of(a, u.b);
     for (int row = rank; row < ROWS && tile * ROWS + row < a.R; row += a.splits) {
         const int gr = tile * ROWS + row, i = token_of(a, gr);
         T* out = reinterpret_cast<T*>(a.p.o) + u.b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - token_of(a, gr) * a.G) * a.p.o_strides.head +
@@ -887,11 +939,11 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_
     const int gr = tile * tile_rows + row;
     if (row >= a.rows || gr >= a.R) return;
     const int2 who = a.shares[blockIdx.x];
-    const int steps = steps_of(a, b), i = token_of(a, gr);
+    const int len = length_of(a, b), steps = steps_for(a, len), i = token_of(a, gr);
     T* out = reinterpret_cast<T*>(a.p.o) + b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - i * a.G) * a.p.o_strides.head +
              (int64_t)i * a.p.o_strides.seq;
     float* lse = a.p.lse ? a.p.lse + ((int64_t)b * a.p.Hq + h * a.G + gr - i * a.G) * a.p.Sq + i : nullptr;
-    const int n = new_tokens(a.p.new_len, b, a.p.Sq), len = a.p.kv_len ? a.p.kv_len[b] : a.c.S;
+    const int n = new_tokens(a.p.new_len, b, a.p.Sq);
     const int first = kWide ? tid : lane;
     if (steps == 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
         for (int d = first; d < D; d += kWide ? kThreads : 32) st_value(out + d, 0.f);
@@ -1040,7 +1092,7 @@ int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_dec
     auto on = [&](const void* ptr, const ltca_strides& st, int to) {
         return !((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(st.batch * es) | (uintptr_t)(st.head * es) | (uintptr_t)(st.seq * es)) & (to - 1));
     };
-    a.vec_q = on(p->q, p->q_strides, 4 * es);
+    a.vec_q = on(p->q, p->q_strides, 16);
     a.vec_o = on(p->o, p->o_strides, 4 * es);
     // new tokens that 8 NT rows in a line reach
     const int span = (8 * s.nt - 1 + a.G - 1) / a.G + 1;
