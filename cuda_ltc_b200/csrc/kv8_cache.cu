@@ -18,7 +18,7 @@ struct AppendArgs {
     ltca_kv8_append_params p;
     int nb, spans;              // blocks of a sequence; of them at most this many are touched
     int vec;                    // rows of k and v start on 16-byte boundaries
-    int64_t items;
+    uint32_t items;             // tensors, heads and sequences
 };
 
 // The bounds' two ends of eight codes (as four pairs of fp16), NaN at both.
@@ -63,33 +63,74 @@ __device__ __forceinline__ Piece8b load_piece(const __nv_bfloat16* x, bool vec) 
     }
     return r;
 }
+// The largest magnitude as bits; an infinity or NaN shows as 0x7f800000 or more.
+__device__ __forceinline__ void largest(const Piece8f& p, uint32_t& m) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(p.v[i]) & 0x7fffffffu);
+}
+__device__ __forceinline__ void largest(const Piece8b& p, uint32_t& m) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t = __vmaxu2(t, p.v[i] & 0x7fff7fffu);
+    m = max(m, max(t << 16, t & 0xffff0000u));
+}
+// The smallest and the largest of each channel so far.
+struct Ends8f {
+    float lo[8], hi[8];
+    __device__ __forceinline__ Ends8f() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { lo[i] = INFINITY; hi[i] = -INFINITY; }
+    }
+    __device__ __forceinline__ void add(const Piece8f& p) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { lo[i] = fminf(lo[i], p.v[i]); hi[i] = fmaxf(hi[i], p.v[i]); }
+    }
+    __device__ __forceinline__ float low(int i) const { return lo[i]; }
+    __device__ __forceinline__ float high(int i) const { return hi[i]; }
+};
+struct Ends8b {
+    __nv_bfloat162 lo[4], hi[4];
+    __device__ __forceinline__ Ends8b() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { lo[i] = __float2bfloat162_rn(INFINITY); hi[i] = __float2bfloat162_rn(-INFINITY); }
+    }
+    __device__ __forceinline__ void add(const Piece8b& p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&p.v[i]);
+            lo[i] = __hmin2(lo[i], x);
+            hi[i] = __hmax2(hi[i], x);
+        }
+    }
+    __device__ __forceinline__ float low(int i) const { return i & 1 ? __high2float(lo[i >> 1]) : __low2float(lo[i >> 1]); }
+    __device__ __forceinline__ float high(int i) const { return i & 1 ? __high2float(hi[i >> 1]) : __low2float(hi[i >> 1]); }
+};
 __device__ __forceinline__ float value_of(const Piece8f& p, int i) { return p.v[i]; }
 __device__ __forceinline__ float value_of(const Piece8b& p, int i) {
     return __uint_as_float(i & 1 ? p.v[i >> 1] & 0xffff0000u : p.v[i >> 1] << 16);
 }
-template <typename T> struct PieceOf { using type = Piece8f; };
-template <> struct PieceOf<__nv_bfloat16> { using type = Piece8b; };
+template <typename T> struct PieceOf { using type = Piece8f; using ends = Ends8f; };
+template <> struct PieceOf<__nv_bfloat16> { using type = Piece8b; using ends = Ends8b; };
 
 // P pieces per thread of a team of TEAM hold a block's new rows.
 template <typename T, int TEAM, int P>
 __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int kTeamWarps = TEAM / 32;
-    __shared__ uint32_t sm_max[kTeamWarps];
+    __shared__ uint32_t sm_max[2][kTeamWarps];
     __shared__ __half2 sm_lo[kTeamWarps][64], sm_hi[kTeamWarps][64];        // by pairs of channels
     grid_dependency_wait();
     const int tid = TEAM == 32 ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31, warp = TEAM == 32 ? 0 : threadIdx.x >> 5;
-    // the two tensors' blocks side by side, then the heads, then a sequence's blocks
-    const int64_t item = TEAM == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    // x: the two tensors side by side, then the heads, then the sequences; y: a sequence's blocks
+    const uint32_t item = TEAM == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (item >= a.items) return;
     const bool is_v = item & 1;
-    const int span = (int)((item >> 1) % a.spans);
-    const int64_t pair = (item >> 1) / a.spans;
-    const int b = (int)(pair / a.c.H), h = (int)(pair % a.c.H), D = a.c.D;
-    const int log_chunks = 31 - __clz(D) - 3, chunks = 1 << log_chunks;       // pieces of a row
+    const uint32_t pair = item >> 1;
+    const int b = (int)(pair / (uint32_t)a.c.H), h = (int)(pair - (uint32_t)b * a.c.H), D = a.c.D;
+    const int log_chunks = 31 - __clz(D) - 3, chunks = 1 << log_chunks, log_block = 31 - __clz(a.c.block);       // pieces of a row
     const int n = new_tokens(a.p.new_len, b, a.p.n);
     const int64_t end = a.p.kv_len[b], first = end - n;
     const int64_t lo_pos = first > 0 ? first : 0, hi_pos = end < a.c.S ? end : a.c.S;       // positions that are written
-    const int64_t j = lo_pos / a.c.block + span, row0 = j * a.c.block;
+    const int64_t j = (lo_pos >> log_block) + blockIdx.y, row0 = j << log_block;
     if (lo_pos >= hi_pos || row0 >= hi_pos) return;
     const int from = (int)(lo_pos > row0 ? lo_pos - row0 : 0), to = (int)(hi_pos - row0 < a.c.block ? hi_pos - row0 : a.c.block);
 
@@ -98,7 +139,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
     // token of the block's row r: row0 + r - first
     const T* x = reinterpret_cast<const T*>(is_v ? a.p.v : a.p.k) + b * xs.batch + h * xs.head + (row0 - first) * xs.seq + chunk * 8;
     uint8_t* code = reinterpret_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + b * cs.batch + h * cs.head + row0 * cs.seq + chunk * 8;
-    const int64_t at = pair * a.nb + j;
+    const int64_t at = (int64_t)pair * a.nb + j;
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + at;
     const float old = from > 0 ? *scale : 0.f;
     const bool bounded = a.c.bounds && !is_v;
@@ -111,18 +152,34 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
         const int row = from + ((tid + i * TEAM) >> log_chunks);
         if (row < to) piece[i] = load_piece(x + (int64_t)row * xs.seq, a.vec != 0);
     }
+    typename PieceOf<T>::ends ends;
 #pragma unroll
     for (int i = 0; i < P; ++i)
         if (from + ((tid + i * TEAM) >> log_chunks) < to) {
-#pragma unroll
-            for (int y = 0; y < 8; ++y) most = max(most, finite_abs_bits(value_of(piece[i], y)));
+            largest(piece[i], most);
+            if (bounded) ends.add(piece[i]);
         }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if constexpr (TEAM > 32) {
-        if (lane == 0) sm_max[warp] = most;
-        __syncthreads();
+    auto of_team = [&](uint32_t x, int turn) {
+        x = __reduce_max_sync(0xffffffffu, x);
+        if constexpr (TEAM > 32) {
+            if (lane == 0) sm_max[turn][warp] = x;
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kTeamWarps; ++i) most = max(most, sm_max[i]);
+            for (int i = 0; i < kTeamWarps; ++i) x = max(x, sm_max[turn][i]);
+        }
+        return x;
+    };
+    most = of_team(most, 0);
+    const bool special = most >= 0x7f800000u;                     // infinities and NaN do not count
+    if (special) {
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            if (from + ((tid + i * TEAM) >> log_chunks) < to) {
+#pragma unroll
+                for (int y = 0; y < 8; ++y) most = max(most, finite_abs_bits(value_of(piece[i], y)));
+            }
+        most = of_team(most, 1);
     }
     const int e = e4m3_exponent(most);
     const float need = pow2(e), now = fmaxf(old, need);
@@ -140,7 +197,17 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
             for (int y = 0; y < 4; ++y) w[y] = to_e4m3x2(value_of(piece[i], 2 * y) * up, value_of(piece[i], 2 * y + 1) * up);
             const uint2 c = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
             *reinterpret_cast<uint2*>(code + (int64_t)row * cs.seq) = c;
-            if (bounded) widen(lo, hi, c);
+            if (bounded && special) widen(lo, hi, c);
+        }
+    }
+    if (bounded && !special && from + (tid >> log_chunks) < to) {
+        // rounding keeps the order: the ends of the codes are the codes of the ends
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t l = e4m3x2_to_half2(to_e4m3x2(ends.low(2 * i) * up, ends.low(2 * i + 1) * up));
+            const uint32_t h = e4m3x2_to_half2(to_e4m3x2(ends.high(2 * i) * up, ends.high(2 * i + 1) * up));
+            lo[i] = *reinterpret_cast<const __half2*>(&l);
+            hi[i] = *reinterpret_cast<const __half2*>(&h);
         }
     }
     // The older rows: rounded again where the scale has grown, and looked at for the bounds, which thereby are those of the live
@@ -287,9 +354,7 @@ bool rows_on_16(const void* p, const ltca_strides& s, int es) {
 
 template <typename T, int TEAM, int P>
 int launch_team(ltca_ctx* ctx, const AppendArgs& a) {
-    const int64_t ctas = TEAM == 32 ? (a.items + 3) / 4 : a.items;
-    if (ctas > 0x7fffffff) return fail(ctx, LTCA_ERR_INVALID, "append: too many tokens for one call");
-    const dim3 grid((unsigned)ctas);
+    const dim3 grid(TEAM == 32 ? (a.items + 3) / 4 : a.items, (unsigned)a.spans);
     LTCA_CUDA_OK(ctx, launch_dependent(kv8_append_kernel<T, TEAM, P>, grid, dim3(TEAM == 32 ? 128 : TEAM), 0, ctx->stream, a));
     return LTCA_OK;
 }
@@ -315,7 +380,8 @@ int launch_kv8_append(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_app
     const int64_t spans = ((int64_t)p->n + c->block - 2) / c->block + 1;
     AppendArgs a{*c, *p, nb, (int)(spans < nb ? spans : nb), 0, 0};
     a.vec = rows_on_16(p->k, p->k_strides, es) && rows_on_16(p->v, p->v_strides, es);
-    a.items = (int64_t)c->B * c->H * a.spans * 2;
+    if (a.spans > 65535) return fail(ctx, LTCA_ERR_UNSUPPORTED, "append: %d tokens in blocks of %d are too many for one call", p->n, c->block);
+    a.items = (uint32_t)c->B * (uint32_t)c->H * 2u;
     return p->dtype == LTCA_BF16 ? launch_append<__nv_bfloat16>(ctx, a) : launch_append<float>(ctx, a);
 }
 

@@ -27,7 +27,7 @@ int check_cache(ltca_ctx* ctx, const ltca_kv8_cache* c, bool k, bool v) {
         return fail(ctx, LTCA_ERR_INVALID, "bad cache shape B=%d H=%d S=%d", c->B, c->H, c->S);
     // positions and what the kernels add to them stay in 32 bits
     if (c->S > (1 << 30)) return fail(ctx, LTCA_ERR_UNSUPPORTED, "the capacity is above 2^30 tokens");
-    if ((int64_t)c->B * c->H > 0x7fffffff) return fail(ctx, LTCA_ERR_INVALID, "B * H is above 2^31 - 1");
+    if ((int64_t)c->B * c->H >= 1 << 30) return fail(ctx, LTCA_ERR_INVALID, "B * H is 2^30 or more");
     if (c->D != 32 && c->D != 64 && c->D != 128)
         return fail(ctx, LTCA_ERR_UNSUPPORTED, "the 8-bit cache supports head_dim 32, 64, 128 (got %d)", c->D);
     if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
