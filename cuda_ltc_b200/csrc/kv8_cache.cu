@@ -147,15 +147,18 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
 
     typename PieceOf<T>::type piece[P];
     uint32_t most = 0;
+    // a thread's rows: row0, and every (TEAM / chunks)th from there
+    const int my_row = from + (tid >> log_chunks), rows = TEAM >> log_chunks;
+    const int64_t x_step = rows * xs.seq, c_step = rows * cs.seq;
+    x += my_row * xs.seq;
+    code += my_row * cs.seq;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int row = from + ((tid + i * TEAM) >> log_chunks);
-        if (row < to) piece[i] = load_piece(x + (int64_t)row * xs.seq, a.vec != 0);
-    }
+    for (int i = 0; i < P; ++i)
+        if (my_row + i * rows < to) piece[i] = load_piece(x + i * x_step, a.vec != 0);
     typename PieceOf<T>::ends ends;
 #pragma unroll
     for (int i = 0; i < P; ++i)
-        if (from + ((tid + i * TEAM) >> log_chunks) < to) {
+        if (my_row + i * rows < to) {
             largest(piece[i], most);
             if (bounded) ends.add(piece[i]);
         }
@@ -175,7 +178,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
         most = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i)
-            if (from + ((tid + i * TEAM) >> log_chunks) < to) {
+            if (my_row + i * rows < to) {
 #pragma unroll
                 for (int y = 0; y < 8; ++y) most = max(most, finite_abs_bits(value_of(piece[i], y)));
             }
@@ -190,17 +193,16 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
     for (int i = 0; i < 4; ++i) { lo[i] = __float2half2_rn(448.f); hi[i] = __float2half2_rn(-448.f); }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int row = from + ((tid + i * TEAM) >> log_chunks);
-        if (row < to) {
+        if (my_row + i * rows < to) {
             uint32_t w[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) w[y] = to_e4m3x2(value_of(piece[i], 2 * y) * up, value_of(piece[i], 2 * y + 1) * up);
             const uint2 c = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-            *reinterpret_cast<uint2*>(code + (int64_t)row * cs.seq) = c;
+            *reinterpret_cast<uint2*>(code + i * c_step) = c;
             if (bounded && special) widen(lo, hi, c);
         }
     }
-    if (bounded && !special && from + (tid >> log_chunks) < to) {
+    if (bounded && !special && my_row < to) {
         // rounding keeps the order: the ends of the codes are the codes of the ends
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -214,9 +216,10 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) kv8_append_kernel(con
     // keys whatever became of earlier ones (tokens that were taken back, say).
     if (grown || (bounded && from > 0)) {
         const float by = old / now;
+        code -= from * cs.seq;                                    // rows from the block's first on
 #pragma unroll 4
-        for (int i = tid; (i >> log_chunks) < from; i += TEAM) {
-            uint2* dst = reinterpret_cast<uint2*>(code + (int64_t)(i >> log_chunks) * cs.seq);
+        for (int i = 0; i * rows + (tid >> log_chunks) < from; ++i) {
+            uint2* dst = reinterpret_cast<uint2*>(code + i * c_step);
             uint2 c = *dst;
             if (grown) {
                 uint32_t w[4];
@@ -364,10 +367,10 @@ int launch_append(ltca_ctx* ctx, const AppendArgs& a) {
     if (a.p.n <= 8) return a.p.n <= 2 ? launch_team<T, 32, 1>(ctx, a) : launch_team<T, 32, 4>(ctx, a);
     switch (a.c.block * a.c.D / 8) {
         case 64: return launch_team<T, 64, 1>(ctx, a);
-        case 128: return launch_team<T, 128, 1>(ctx, a);
-        case 256: return launch_team<T, 256, 1>(ctx, a);
-        case 512: return launch_team<T, 256, 2>(ctx, a);
-        case 1024: return launch_team<T, 256, 4>(ctx, a);
+        case 128: return launch_team<T, 64, 2>(ctx, a);
+        case 256: return launch_team<T, 64, 4>(ctx, a);
+        case 512: return launch_team<T, 128, 4>(ctx, a);
+        case 1024: return launch_team<T, 128, 8>(ctx, a);
         default: return launch_team<T, 256, 8>(ctx, a);                       // 2048: 128 tokens of 128 channels
     }
 }
