@@ -339,6 +339,9 @@ SELECTS = [
     (1, 2, 8, 1, 20000, 64, 16, [19985], 100, 2, 3), (4, 8, 2, 1, 300, 32, 128, [300, 129, 128, 1], 2, 1, 1),
     (1, 1, 2, 1, 640, 64, 32, [2000000000], 64, 0, 64), (1, 3, 5, 5, 4100, 64, 16, [4099], 256, 0, 1),
     (2, 1, 1, 1, 300, 64, 16, [-4, 300], 3, 3, 0),
+    (2, 2, 2, 1, 300000, 32, 16, [300000, 270001], 77, 1, 1),       # more blocks than one CTA goes through
+    (1, 1, 40, 1, 2000, 64, 16, [1999], 33, 1, 1),                  # more rows than are in shared memory at once
+    (20, 16, 1, 1, 500, 32, 16, None, 2, 1, 1),                     # a CTA alone; no choice is left
 ]
 
 
