@@ -188,12 +188,15 @@ template <typename T, int D, bool kWide, typename Part>
 __device__ __forceinline__ void join_row(int parts, Part part, float (*sm_o)[D], T* out, float* lse) {
     constexpr int E = D / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float M = kNone, L = 0.f, top = -INFINITY;
-    for (int k = lane; k < parts; k += 32) M = fmaxf(M, part(k)[0]);
+    // lane: a share
+    float4 mine = make_float4(kNone, 0.f, 0.f, 0.f);
+    if (lane < parts) mine = *reinterpret_cast<const float4*>(part(lane));
+    float M = mine.x, L = 0.f, top = -INFINITY;
+    for (int k = lane + 32; k < parts; k += 32) M = fmaxf(M, part(k)[0]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
     for (int k = lane; k < parts; k += 32) {
-        const float4 x = *reinterpret_cast<const float4*>(part(k));
+        const float4 x = k < 32 ? mine : *reinterpret_cast<const float4*>(part(k));
         L += x.z * exp2_fast(x.x - M);
         top = fmaxf(top, (x.x - M) + x.y);
     }
@@ -205,18 +208,23 @@ __device__ __forceinline__ void join_row(int parts, Part part, float (*sm_o)[D],
     float sum[E];
 #pragma unroll
     for (int x = 0; x < E; ++x) sum[x] = 0.f;
-#pragma unroll 4
-    for (int k = kWide ? warp : 0; k < parts; k += kWide ? kWarps : 1) {
-        const float* src = part(k);
-        const float by = exp2_fast((src[0] - M) + src[1] - top);
-        if constexpr (E == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(src + 4 + lane * 4);
-            sum[0] = fmaf(x.x, by, sum[0]); sum[1] = fmaf(x.y, by, sum[1]); sum[2] = fmaf(x.z, by, sum[2]); sum[3] = fmaf(x.w, by, sum[3]);
-        } else if constexpr (E == 2) {
-            const float2 x = *reinterpret_cast<const float2*>(src + 4 + lane * 2);
-            sum[0] = fmaf(x.x, by, sum[0]); sum[1] = fmaf(x.y, by, sum[1]);
-        } else {
-            sum[0] = fmaf(src[4 + lane], by, sum[0]);
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+        if (k0 && k0 + lane < parts) mine = *reinterpret_cast<const float4*>(part(k0 + lane));
+        const float weight = exp2_fast((mine.x - M) + mine.y - top);
+        const int n = min(parts - k0, 32);
+#pragma unroll 8
+        for (int k = kWide ? warp : 0; k < n; k += kWide ? kWarps : 1) {
+            const float* src = part(k0 + k);
+            const float by = __shfl_sync(0xffffffffu, weight, k);
+            if constexpr (E == 4) {
+                const float4 x = *reinterpret_cast<const float4*>(src + 4 + lane * 4);
+                sum[0] = fmaf(x.x, by, sum[0]); sum[1] = fmaf(x.y, by, sum[1]); sum[2] = fmaf(x.z, by, sum[2]); sum[3] = fmaf(x.w, by, sum[3]);
+            } else if constexpr (E == 2) {
+                const float2 x = *reinterpret_cast<const float2*>(src + 4 + lane * 2);
+                sum[0] = fmaf(x.x, by, sum[0]); sum[1] = fmaf(x.y, by, sum[1]);
+            } else {
+                sum[0] = fmaf(src[4 + lane], by, sum[0]);
+            }
         }
     }
     if constexpr (kWide) {
@@ -934,11 +942,12 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_
     __shared__ float sm_o[kWide ? kWarps : 1][D];
     grid_dependency_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per_b = a.c.H * a.tiles, unit = (int)(blockIdx.x % (unsigned)per_b), b = (int)(blockIdx.x / (unsigned)per_b);
-    const int tile = tile_of(a, unit), h = head_of(a, unit), row = kWide ? blockIdx.y : blockIdx.y * kWarps + warp;
-    const int gr = tile * tile_rows + row;
-    if (row >= a.rows || gr >= a.R) return;
-    const int2 who = a.shares[blockIdx.x];
+    const uint32_t per_b = a.c.H * a.tiles, at = kWide ? blockIdx.x : blockIdx.x * kWarps + warp;      // rows of all units
+    const uint32_t place = a.rows == 1 ? at : at / (uint32_t)a.rows;
+    const int row = (int)(at - place * a.rows), b = (int)(place / per_b), unit = (int)(place - b * per_b);
+    const int tile = tile_of(a, unit), h = head_of(a, unit), gr = tile * tile_rows + row;
+    if (b >= a.c.B || gr >= a.R) return;
+    const int2 who = a.shares[place];
     const int len = length_of(a, b), steps = steps_for(a, len), i = token_of(a, gr);
     T* out = reinterpret_cast<T*>(a.p.o) + b * a.p.o_strides.batch + (int64_t)(h * a.G + gr - i * a.G) * a.p.o_strides.head +
              (int64_t)i * a.p.o_strides.seq;
@@ -1028,8 +1037,9 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
         // a CTA for each row where a unit has many shares
         const bool wide = a.warps > 16 * units;
         auto join = wide ? kv8_decode_join_kernel<T, D, true> : kv8_decode_join_kernel<T, D, false>;
-        const dim3 rows((unsigned)units, (unsigned)(wide ? a.rows : (a.rows + kWarps - 1) / kWarps));
-        LTCA_CUDA_OK(ctx, launch_dependent(join, dim3(rows), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
+        const int64_t rows = units * a.rows;
+        const dim3 joins((unsigned)(wide ? rows : (rows + kWarps - 1) / kWarps));
+        LTCA_CUDA_OK(ctx, launch_dependent(join, dim3(joins), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
         return LTCA_OK;
     }
     cudaLaunchConfig_t cfg;
@@ -1078,7 +1088,7 @@ size_t kv8_decode_workspace(const ltca_kv8_cache* c, const ltca_kv8_decode_param
 
 int launch_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     const Plan s = plan_of(c, p);
-    if ((int64_t)c->B * c->H * s.tiles > 0x7fffffff) return fail(ctx, LTCA_ERR_INVALID, "too many rows of queries for one call");
+    if ((int64_t)c->B * c->H * s.tiles * s.rows > 0x7fffffff) return fail(ctx, LTCA_ERR_INVALID, "too many rows of queries for one call");
     if (p->blocks && (int64_t)p->n_blocks * c->block > (1 << 30))
         return fail(ctx, LTCA_ERR_UNSUPPORTED, "the listed blocks hold more than 2^30 tokens");
     DecodeArgs a;
