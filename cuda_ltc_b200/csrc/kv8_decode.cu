@@ -40,7 +40,7 @@ constexpr int kHead = 48;                   // a step's positions and scales
 constexpr int kMaxCluster = 8;              // CTAs that join their shares through shared memory
 constexpr int kClusterSteps = 8;            // of a warp there, at most
 constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do
-constexpr int kUnitCost = 2;                // what a unit costs beside its steps, in steps
+constexpr int kUnitCost = 3;                // what a unit costs beside its steps, in steps
 constexpr int kNowhere = 0x7fffffff;        // the position of a group that is not there
 constexpr float kNone = -3.402823466e38f;   // the reference of a row that has seen no key
 constexpr float kLimit = 16384.f;           // largest weight before the references move
@@ -935,13 +935,15 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     if (a.splits > 1) cluster.sync();                               // until nobody reads this CTA's shared memory
 }
 
-// The warps' shares of a unit's rows joined; what no warp or a single one has seen is zeros, or finished already.  kWide: a CTA
-// per row, for many shares; else a warp.
+// The warps' shares of a unit's rows joined; what no warp or a single one has seen is zeros, or finished already.  A warp takes a
+// row; where units have many shares (kWide) a CTA does, whose threads first weigh the shares side by side.
+constexpr int kWideThreads = 512;
 template <typename T, int D, bool kWide>
-__global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_constant__ DecodeArgs a, int tile_rows) {
-    __shared__ float sm_o[kWide ? kWarps : 1][D];
+__global__ void __launch_bounds__(kWide ? kWideThreads : kThreads) kv8_decode_join_kernel(const __grid_constant__ DecodeArgs a, int tile_rows) {
+    constexpr int kTeam = kWide ? kWideThreads : 32, E = D / 32;
+    __shared__ float sm_o[kWide ? kWideThreads / 32 : 1][D], sm_w[kWide ? kWideThreads : 1], sm_x[3][kWideThreads / 32];
     grid_dependency_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, first = kWide ? tid : lane;
     const uint32_t per_b = a.c.H * a.tiles, at = kWide ? blockIdx.x : blockIdx.x * kWarps + warp;      // rows of all units
     const uint32_t place = a.rows == 1 ? at : at / (uint32_t)a.rows;
     const int row = (int)(at - place * a.rows), b = (int)(place / per_b), unit = (int)(place - b * per_b);
@@ -953,16 +955,72 @@ __global__ void __launch_bounds__(kThreads) kv8_decode_join_kernel(const __grid_
              (int64_t)i * a.p.o_strides.seq;
     float* lse = a.p.lse ? a.p.lse + ((int64_t)b * a.p.Hq + h * a.G + gr - i * a.G) * a.p.Sq + i : nullptr;
     const int n = new_tokens(a.p.new_len, b, a.p.Sq);
-    const int first = kWide ? tid : lane;
     if (steps == 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
-        for (int d = first; d < D; d += kWide ? kThreads : 32) st_value(out + d, 0.f);
+        for (int d = first; d < D; d += kTeam) st_value(out + d, 0.f);
         if (first == 0 && lse) *lse = -INFINITY;
         return;
     }
     if (who.y == 0) return;
     // the first share is the last thing that its warp did, the others the first
+    const int parts = who.y + 1;
     auto part = [&](int k) -> const float* { return a.partial + ((int64_t)(2 * (who.x + k) + (k == 0 ? 1 : 0)) * a.rows + row) * (D + 4); };
-    join_row<T, D, kWide>(who.y + 1, part, sm_o, out, lse);
+    if constexpr (!kWide) {
+        join_row<T, D, false>(parts, part, sm_o, out, lse);
+    } else {
+        float4 mine = make_float4(kNone, 0.f, 0.f, 0.f);
+        if (tid < parts) mine = *reinterpret_cast<const float4*>(part(tid));
+        float M = mine.x, L = 0.f, top = -INFINITY;
+        for (int k = tid + kTeam; k < parts; k += kTeam) M = fmaxf(M, part(k)[0]);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        if (lane == 0) sm_x[0][warp] = M;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kTeam / 32; ++w) M = fmaxf(M, sm_x[0][w]);
+        for (int k = tid; k < parts; k += kTeam) {
+            const float4 x = k < kTeam ? mine : *reinterpret_cast<const float4*>(part(k));
+            L += x.z * exp2_fast(x.x - M);
+            top = fmaxf(top, (x.x - M) + x.y);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            L += __shfl_xor_sync(0xffffffffu, L, off);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        }
+        if (lane == 0) { sm_x[1][warp] = L; sm_x[2][warp] = top; }
+        __syncthreads();
+        L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kTeam / 32; ++w) { L += sm_x[1][w]; top = fmaxf(top, sm_x[2][w]); }
+        float sum[E];
+#pragma unroll
+        for (int x = 0; x < E; ++x) sum[x] = 0.f;
+        for (int k0 = 0; k0 < parts; k0 += kTeam) {
+            if (k0) {
+                if (k0 + tid < parts) mine = *reinterpret_cast<const float4*>(part(k0 + tid));
+                __syncthreads();
+            }
+            sm_w[tid] = exp2_fast((mine.x - M) + mine.y - top);
+            __syncthreads();
+            const int m = min(parts - k0, kTeam);
+#pragma unroll 4
+            for (int k = warp; k < m; k += kTeam / 32) {
+                const float* src = part(k0 + k) + 4 + lane;
+#pragma unroll
+                for (int x = 0; x < E; ++x) sum[x] = fmaf(src[32 * x], sm_w[k], sum[x]);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < E; ++x) sm_o[warp][lane + 32 * x] = sum[x];
+        __syncthreads();
+        if (tid < D) {
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < kTeam / 32; ++w) y += sm_o[w][tid];
+            st_value(out + tid, L == 0.f ? 0.f : y * (pow2((int)top - 6) / L));
+        }
+        if (tid == 0 && lse) *lse = L == 0.f ? -INFINITY : (M == kNone ? 0.f : M * 0.693147181f) + logf(L);
+    }
 }
 
 // How a call is cut up; a function of the problem alone, so that the size query and the launch agree.
@@ -1039,7 +1097,7 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
         auto join = wide ? kv8_decode_join_kernel<T, D, true> : kv8_decode_join_kernel<T, D, false>;
         const int64_t rows = units * a.rows;
         const dim3 joins((unsigned)(wide ? rows : (rows + kWarps - 1) / kWarps));
-        LTCA_CUDA_OK(ctx, launch_dependent(join, dim3(joins), dim3(kThreads), 0, ctx->stream, a, 8 * NT));
+        LTCA_CUDA_OK(ctx, launch_dependent(join, dim3(joins), dim3(wide ? kWideThreads : kThreads), 0, ctx->stream, a, 8 * NT));
         return LTCA_OK;
     }
     cudaLaunchConfig_t cfg;
