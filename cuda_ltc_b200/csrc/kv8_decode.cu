@@ -102,6 +102,23 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d += A (B's terms, low-order first).  The tensor pipe cuts its running sums off instead of rounding them, which over the products of
+// a long sequence comes to 1e-6 of the result; with fp32 rows every product is therefore summed from zero and added by the FMA
+// pipe, to nearest (8 sequences of up to 16384 keys against 64 bits: 1.4e-6 without, 3.3e-7 with, for 5 to 9 % of the time with up to
+// eight rows and up to 30 % with sixteen).
+template <int kTerms>
+__device__ __forceinline__ void add_product(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b0)[kTerms],
+                                            const uint32_t (&b1)[kTerms]) {
+    if constexpr (kTerms == 1) {
+        mma(d, a0, a1, a2, a3, b0[0], b1[0]);
+    } else {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = kTerms - 1; i >= 0; --i) mma(x, a0, a1, a2, a3, b0[i], b1[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] += x[i];
+    }
+}
 // An 8 x 8 matrix of 16-bit values, two of a row in each lane, transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t r;
@@ -641,12 +658,16 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                     codes_to_half2(w[g][0][i], a0, a2);
                     codes_to_half2(w[g][1][i], a1, a3);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+                    for (int t = 0; t < NT; ++t) {
+                        uint32_t b0[kTerms], b1[kTerms];
 #pragma unroll
                         for (int x = 0; x < kTerms; ++x) {
                             const uint2 q = q_at(t, x, part * kWords + i);
-                            mma(s[g][t], a0, a1, a2, a3, q.x, q.y);
+                            b0[x] = q.x;
+                            b1[x] = q.y;
                         }
+                        add_product<kTerms>(s[g][t], a0, a1, a2, a3, b0, b1);
+                    }
                 }
         }
         // s[g][t][0], [1]: key r of the group with rows 2c, 2c + 1; [2], [3]: key r + 8.  The scores are s ck.
@@ -813,9 +834,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 codes_to_half2(__byte_perm(v[0][i >> 1], v[1][i >> 1], sel), a0, a1);
                 codes_to_half2(__byte_perm(v[2][i >> 1], v[3][i >> 1], sel), a2, a3);
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int x = 0; x < kTerms; ++x) mma(o[t][i], a0, a1, a2, a3, w0[t][x], w1[t][x]);
+                for (int t = 0; t < NT; ++t) add_product<kTerms>(o[t][i], a0, a1, a2, a3, w0[t], w1[t]);
             }
         }
     };

@@ -478,6 +478,56 @@ def test_calls_on_two_streams_and_contexts(ctx):
         c.close()
 
 
+def test_two_captured_graphs_of_one_context(ctx):
+    """Calls that join their shares through scratch, captured into two graphs and replayed side by side: each graph has scratch of
+    its own, which a larger call in between does not take away."""
+    B, H, S, D = 2, 2, 20000, 64
+    refs = [filled(B, H, S, D, 64, i) for i in range(2)]
+    caches = [device_cache(r) for r in refs]
+    qs = [queries(B, 2 * H, 1, D, "f32", 30 + i) for i in range(2)]
+    want = [ctx.kv8_decode(q, c) for q, c in zip(qs, caches)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for q, c, s in zip(qs, caches, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ctx.set_stream(s)
+            outs.append(ctx.kv8_decode(q, c))
+        graphs.append(g)
+    ctx.set_stream(torch.cuda.current_stream())
+    big = filled(4, 8, 20000, D, 64, 3)
+    ctx.kv8_decode(queries(4, 64, 1, D, "f32", 5), device_cache(big))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for got, ref in zip(outs, want):
+        assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+@pytest.mark.parametrize("case", [
+    # B, H, G, Sq, S, D            fp32 queries over many keys: the sums do not drift
+    (4, 4, 2, 1, 16000, 128), (2, 2, 4, 2, 30000, 32), (60, 8, 1, 1, 2000, 64)])
+def test_decode_in_fp32_stays_below_1e_6(ctx, case):
+    """In the 2-norm over all of the result against 64 bits.  Each fp32 rounding is off by 2^-24 of its sum at most and in either
+    direction, so that the roundings of a row's sums add up like the root of their number at most: for 16000 keys in warps that
+    take 64 and more of them, 2^-24 sqrt(500) = 1.3e-6 at the very worst of a row, a third of it in the mean of uniform errors;
+    the fp16 terms (2^-22) and exponentials (2^-22) come to less."""
+    B, H, G, Sq, S, D = case
+    ref = filled(B, H, S, D, 64, 12, spread=2.0)
+    q = queries(B, H * G, Sq, D, "f32", 6)
+    o, _ = ctx.kv8_decode(q, device_cache(ref))
+    k, v = (torch.from_numpy(x).cuda() for x in ref.values())
+    x = q.double().reshape(B, H, G * Sq, D) @ k.transpose(2, 3) * D ** -0.5
+    seen = torch.arange(S, device="cuda")[None] <= S - Sq + torch.arange(Sq, device="cuda")[:, None]
+    x = x.view(B, H, G, Sq, S).masked_fill(~seen, -float("inf")).view(B, H, G * Sq, S)
+    want = (torch.softmax(x, 3) @ v).view(B, H * G, Sq, D)
+    assert ((o.double() - want).norm() / want.norm()).item() < 1e-6
+
+
 def test_results_repeat_bit_for_bit(ctx):
     ref = filled(3, 4, 3000, 128, 64, 5)
     cache, q = device_cache(ref), queries(3, 16, 2, 128, "f32", 2)
