@@ -51,11 +51,8 @@ template <int D> constexpr int kGroups = step_groups(D);
 template <int D> constexpr int kStepBytes = kGroups<D> * 32 * D;
 template <int D> constexpr int kStages = D == 128 ? 2 : 3;
 // CTAs of an SM, by the registers that NT tiles of 8 rows take
-constexpr int ctas_per_sm(int D, int nt) { return nt == 4 || nt * D >= 256 ? 2 : nt == 1 && D <= 64 ? 4 : 3; }
+constexpr int ctas_per_sm(int D, int nt) { return nt * D >= 256 ? 2 : nt == 1 && D <= 64 ? 4 : 3; }
 template <int D, int NT> constexpr int kCtas = ctas_per_sm(D, NT);
-// Tiles of 8 rows that a warp keeps at most: a stage of the ring has room for the rows of Q, and fp32's two terms of 128 channels
-// leave registers for two.
-constexpr int most_tiles(int es, int D) { return es == 4 && D >= 64 ? 2 : 4; }
 constexpr int kLens = 256;                  // lengths in shared memory
 
 struct DecodeArgs {
@@ -272,7 +269,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
     constexpr bool kQRegs = NT * kTerms * D <= 256;               // Q's fragments stay in registers
     constexpr int ST = kStages<D>, SG = kGroups<D>;
-    constexpr int NG = NT == 4 ? 1 : 2;                           // groups whose products interleave, as the registers allow
+    constexpr int NG = 2;                                         // groups whose products interleave
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) uint2 sm_q[kQRegs ? 1 : kWarps][kQRegs ? 1 : NT][kQRegs ? 1 : kTerms][kQRegs ? 1 : W][32];
     __shared__ __align__(8) uint64_t sm_bar[kWarps][ST];
@@ -493,7 +490,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     int lim_min = 0;
     float o[NT][W][4];
     uint2 qf[kQRegs ? NT : 1][kQRegs ? kTerms : 1][kQRegs ? W : 1];
-    uint64_t mask_row = 0;                                        // the mask's rows of this lane's rows, a byte each
+    uint32_t mask_row = 0;                                        // the mask's rows of this lane's rows, a byte each
     int mask_rows = 0;                                            // that the tile's rows need
     auto clear = [&]() {
 #pragma unroll
@@ -521,7 +518,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) mask_row |= (uint64_t)__shfl_sync(0xffffffffu, at, t * 8 + 2 * c + k) << (8 * (2 * t + k));
+                for (int k = 0; k < 2; ++k) mask_row |= (uint32_t)__shfl_sync(0xffffffffu, at, t * 8 + 2 * c + k) << (8 * (2 * t + k));
             mask_rows = min(a.mask_rows, a.p.Sq - first);
         }
         if constexpr (!kQRegs) __syncwarp();
@@ -609,7 +606,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
         // hides or shows all of a step's keys from all rows is settled here.
         uint32_t word = 0xffffffffu;
         if (a.p.keep_mask) {
-            const float* mask = reinterpret_cast<const float*>(head + kHead) + (g0 & ~1) * 16 + lane;
+            const float* mask = reinterpret_cast<const float*>(head + kHead) + g0 * 16 + lane;
             uint32_t any = 0, all = 0xffffffffu;
             for (int i = 0; i < mask_rows; ++i) {
                 const uint32_t v = __ballot_sync(0xffffffffu, mask[i * SG * 16] != 0.f);
@@ -617,13 +614,12 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 any |= v;
                 all &= v;
             }
-            const uint32_t those = NG == 2 ? 0xffffffffu : 0xffffu << (16 * (g0 & 1));
             uint32_t seen = 0;
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                if (pos[g] != kNowhere) seen |= 0xffffu << (16 * ((g0 + g) & 1));
+                if (pos[g] != kNowhere) seen |= 0xffffu << (16 * g);
             if ((any & seen) == 0) return;
-            if ((all & those) != those) whole = false;
+            if (all != 0xffffffffu) whole = false;
         }
         const unsigned char* body = ring + stage * kStepBytes<D> + g0 * Gr::kBytes;
         float s[NG][NT][4];
@@ -678,13 +674,13 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) ck[g][t][x] = cs[t][x] * k_scale[g];
-        if (!whole || clamped) {
+        if (__builtin_expect(!whole || clamped, 0)) {
             uint32_t bits[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
-                    bits[t][x] = __shfl_sync(0xffffffffu, word, (int)(mask_row >> (8 * (2 * t + x))) & 31) >> r;
+                    bits[t][x] = __shfl_sync(0xffffffffu, word, mask_row >> (8 * (2 * t + x)) & 31) >> r;
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -695,7 +691,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                         float y = s[g][t][x] * ck[g][t][x & 1];
                         if (clamped) y = y > clamp ? clamp : y;                   // (NaN stays)
                         const bool seen = pos[g] != kNowhere && pos[g] + r + key < lim[t][x & 1] &&
-                                          (bits[t][x & 1] >> (16 * ((g0 + g) & 1) + key) & 1);
+                                          (bits[t][x & 1] >> (16 * g + key) & 1);
                         s[g][t][x] = seen ? y : -INFINITY;
                     }
 #pragma unroll
@@ -721,7 +717,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 }
             return top > kLimit;
         };
-        if (__any_sync(0xffffffffu, weigh())) {
+        if (__builtin_expect(__any_sync(0xffffffffu, weigh()), 0)) {
             float lv[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) lv[g] = fmaxf(log2f(v_scale[g]), -110.f);
@@ -786,7 +782,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                     v[x][0] = *reinterpret_cast<const uint32_t*>(src);
                 }
             }
-            if (!whole) {
+            if (__builtin_expect(!whole, 0)) {
                 // NaN among the values counts for the rows that see its key and for no other: it becomes zero, and a product
                 // of "is NaN" with "is seen" says whose sums it reaches.
                 uint32_t nan[4][VW], any = 0;
@@ -897,7 +893,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
             start_unit(ring + stage * kStepBytes<D>);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA writes next where these rows lay
         } else {
-#pragma unroll
+#pragma unroll 1
             for (int g = 0; g < SG; g += NG) step(stage, g);
         }
         __syncwarp();
@@ -1047,7 +1043,8 @@ struct Plan { int nt, tiles, rows, warps, splits; };
 Plan plan_of(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p) {
     const int R = p->Hq / c->H * p->Sq;
     Plan s;
-    s.nt = R <= 8 ? 1 : R <= 16 || most_tiles(elem_size(p->dtype), c->D) == 2 ? 2 : 4;
+    // (four tiles a warp leave the registers no room for two groups at once: 40 rows of 4000 keys of 128 85 us, in two passes 56)
+    s.nt = R <= 8 ? 1 : 2;
     s.tiles = (R + 8 * s.nt - 1) / (8 * s.nt);
     s.rows = R < 8 * s.nt ? R : 8 * s.nt;
     const int64_t units = (int64_t)c->B * c->H * s.tiles;
@@ -1147,8 +1144,6 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
 }
 template <typename T, int D>
 int launch_rows(ltca_ctx* ctx, const DecodeArgs& a, int nt) {
-    if constexpr (most_tiles(sizeof(T), D) == 4)
-        if (nt == 4) return launch<T, D, 4>(ctx, a);
     return nt == 1 ? launch<T, D, 1>(ctx, a) : launch<T, D, 2>(ctx, a);
 }
 template <typename T>

@@ -303,7 +303,7 @@ typedef struct {
     size_t workspace_bytes;
 } ltca_kv8_decode_params;
 int ltca_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decode_params* p);
-/* Room for the shares of rows that several warps work on: 5 to 40 MB for large calls, little for small ones. */
+/* Room for the shares of rows that several warps work on: 5 to 20 MB for large calls, little for small ones. */
 int ltca_kv8_decode_workspace_bytes(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p, size_t* bytes_out);
 
 /*
