@@ -331,6 +331,28 @@ def test_decode_into_given_outputs_of_any_layout(ctx):
     assert big.double().sum().item() == 5.0 * (big.numel() - out.numel())
 
 
+def test_decode_and_read_of_shared_keys(ctx):
+    """Sequences (or heads) that share their keys through a stride of zero: a common prompt."""
+    B, H, S, D = 3, 2, 500, 64
+    one = filled(1, H, S, D, 64, 5)
+    cache = device_cache(one)
+    q = queries(B, 2 * H, 1, D, "bf16", 2)
+    rows = lambda t: t.expand(B, *t.shape[1:]).contiguous()  # noqa: E731
+    shared = ltc.Kv8Cache(cache.k.expand(B, H, S, D), cache.v.expand(B, H, S, D), rows(cache.k_scale), rows(cache.v_scale), None, 64)
+    length = ints([500, 64, 333])
+    got = ctx.kv8_decode(q, shared, kv_len=length)
+    own = ltc.Kv8Cache(*(rows(t.view(torch.uint8)).view(torch.float8_e4m3fn) for t in cache[:2]), shared.k_scale, shared.v_scale, None, 64)
+    want = ctx.kv8_decode(q, own, kv_len=length)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(ctx.kv8_read(shared, kv_len=length)[0], ctx.kv8_read(own, kv_len=length)[0])
+    heads = shared._replace(k=own.k[:, :1].expand(B, H, S, D), k_scale=own.k_scale[:, :1].expand(B, H, -1).contiguous())
+    got = ctx.kv8_decode(q, heads, kv_len=length)
+    want = ctx.kv8_decode(q, heads._replace(k=rows(heads.k.contiguous())), kv_len=length)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(ltc.LtcaError):                               # tokens that share a key are no cache
+        ctx.kv8_decode(q, shared._replace(k=own.k[:, :, :1].expand(B, H, S, D)), kv_len=length)
+
+
 # ---- select ------------------------------------------------------------------------------------
 SELECTS = [
     # B, H, G, Sq, S, D, block, kv_len, count, first, last
