@@ -207,6 +207,8 @@ DECODES = [
     (40, 8, 1, 1, 600, 64, 32, "spread", "bhsd"),
     (5, 16, 2, 1, 1300, 32, 128, "spread", "bhsd"),
     (2, 1, 1, 3, 64, 64, 16, [2000000000, -7], "bhsd"),     # lengths behind the capacity and below zero
+    (8, 8, 4, 1, 900, 128, 64, "spread", "bhsd"),           # clusters of six CTAs a pair
+    (16, 8, 1, 1, 500, 128, 32, "spread", "bshd"),          # of three
 ]
 
 
