@@ -296,6 +296,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
     if (lane < ST) mbar_init(smem_u32(&sm_bar[warp][lane]), 1);
     mbar_fence_init();
     if (tid == 0) sm_abort = 0;
+    __syncthreads();                                              // no warp polls a word or uses a barrier that is not set yet
     grid_dependency_wait();
 
     const int per_b = a.c.H * a.tiles;                            // units of a sequence
