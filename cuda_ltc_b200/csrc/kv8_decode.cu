@@ -37,6 +37,7 @@
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
+#include "kv8_shares.h"
 
 namespace ltca {
 
@@ -984,6 +985,11 @@ __global__ void __launch_bounds__(kWide ? kWideThreads : kThreads) kv8_decode_jo
     if (steps == 0 || i >= n || (a.p.causal && (int64_t)len - n + i + 1 <= 0)) {
         for (int d = first; d < D; d += kTeam) st_value(out + d, 0.f);
         if (first == 0 && lse) *lse = -INFINITY;
+        return;
+    }
+    if (!shares_are_there(who.x, who.y, a.warps)) {               // a warp gave up: the row is unknown
+        for (int d = first; d < D; d += kTeam) st_value(out + d, __int_as_float(0x7fc00000));
+        if (first == 0 && lse) *lse = __int_as_float(0x7fc00000);
         return;
     }
     if (who.y == 0) return;
