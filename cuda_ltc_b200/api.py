@@ -64,7 +64,7 @@ class Context:
         if rc != 0:
             raise LtcaError(rc, "ltca_ctx_create failed (is this an sm_100 GPU?)")
         self.handle = handle
-        self._host = _lib.load_host(LtcaError).Host(handle.value, self.device, sptr.value or 0)
+        self._host = _lib.load_host(LtcaError).Host(handle.value, self.device)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -79,7 +79,7 @@ class Context:
             pass
 
     def set_stream(self, stream: torch.cuda.Stream):
-        self._host.set_stream(stream.cuda_stream)
+        self.lib.ltca_ctx_set_stream(self.handle, C.c_void_p(stream.cuda_stream))
 
     def enable_kernel_timing(self, enable: bool = True):
         """Per-kernel CUDA-event timing of the tensor-pipe backward (benchmark aid)."""

@@ -483,6 +483,12 @@ int ltca_ctx_set_stream(ltca_ctx* ctx, void* stream) {
     return LTCA_OK;
 }
 
+int ltca_ctx_get_stream(const ltca_ctx* ctx, void** stream_out) {
+    if (!ctx || !stream_out) return LTCA_ERR_INVALID;
+    *stream_out = ctx->stream;
+    return LTCA_OK;
+}
+
 void ltca_ctx_destroy(ltca_ctx* ctx) {
     if (!ctx) return;
     for (int i = 0; i < 4; ++i)

@@ -15,6 +15,7 @@
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -44,7 +45,6 @@ struct Host {
     PyObject_HEAD
     ltca_ctx* ctx;
     int device;
-    cudaStream_t stream; // the context's
     at::Tensor* ws;      // scratch, grown on demand and kept
 };
 
@@ -108,8 +108,24 @@ inline int truth(PyObject* o) {
     return v;
 }
 
-inline at::Tensor empty(const Host* h, at::IntArrayRef sizes, at::ScalarType t) {
+inline at::Tensor empty_now(const Host* h, at::IntArrayRef sizes, at::ScalarType t) {
     return at::Tensor(at::detail::empty_cuda(sizes, t, at::Device(at::kCUDA, (c10::DeviceIndex)h->device), std::nullopt));
+}
+// Memory that the context's stream writes.  Where that is not torch's current stream the block is one of the context's stream: the
+// allocator hands out what kernels of the stream that it allocates for may still be using, which only that stream's order makes
+// safe.  `seen`: the caller gets it, and uses it on the current stream; it is not given away again before that has come to its end.
+at::Tensor empty(const Host* h, at::IntArrayRef sizes, at::ScalarType t, bool seen = true) {
+    void* own = nullptr;
+    const auto device = (c10::DeviceIndex)h->device;
+    const c10::cuda::CUDAStream now = c10::cuda::getCurrentCUDAStream(device);
+    if (ltca_ctx_get_stream(h->ctx, &own) != 0 || own == now.stream()) return empty_now(h, sizes, t);
+    at::Tensor r;
+    {
+        c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(own), device));
+        r = empty_now(h, sizes, t);
+    }
+    if (seen) c10::cuda::CUDACachingAllocator::recordStream(r.storage().data_ptr(), now);
+    return r;
 }
 inline PyObject* wrap(at::Tensor t) {
     PyObject* o = THPVariable_Wrap(std::move(t));
@@ -438,10 +454,7 @@ PyObject* kv8_decode(Host* h, PyObject* const* a) {
     // A block of its own for each call, and not the context's scratch: what a captured call was given stays with its graph.
     at::Tensor ws;
     if (need) {
-        ws = empty(h, {(int64_t)need}, at::kByte);
-        const auto mine = c10::cuda::getStreamFromExternal(h->stream, (c10::DeviceIndex)h->device);
-        if (mine.stream() != c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)h->device).stream())
-            c10::cuda::CUDACachingAllocator::recordStream(ws.storage().data_ptr(), mine);
+        ws = empty(h, {(int64_t)need}, at::kByte, false);
         p.workspace = ws.data_ptr();
         p.workspace_bytes = need;
     }
@@ -639,13 +652,6 @@ PyObject* host_workspace(Host* h, PyObject* const* a) {
     return wrap(std::move(ws));
 }
 
-// (address of the stream): the stream that the context's calls enqueue on from now on.
-PyObject* host_set_stream(Host* h, PyObject* const* a) {
-    h->stream = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(word64(a[0])));
-    ltca_ctx_set_stream(h->ctx, h->stream);
-    Py_RETURN_NONE;
-}
-
 // (): the context is gone; later calls fail with LTCA_ERR_INVALID.
 PyObject* host_close(Host* h, PyObject* const*) {
     h->ctx = nullptr;
@@ -688,18 +694,16 @@ PyMethodDef host_methods[] = {
     LTCA_METHOD(fa_fwd, kModuleArgs + 3),
     LTCA_METHOD(fa_bwd, kModuleArgs + 4),
     {"workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<host_workspace, 1>)), METH_FASTCALL, nullptr},
-    {"set_stream", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<host_set_stream, 1>)), METH_FASTCALL, nullptr},
     {"close", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<host_close, 0>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 int host_init(PyObject* self, PyObject* args, PyObject*) {
-    unsigned long long ctx = 0, stream = 0;
+    unsigned long long ctx = 0;
     int device = 0;
-    if (!PyArg_ParseTuple(args, "KiK", &ctx, &device, &stream)) return -1;
+    if (!PyArg_ParseTuple(args, "Ki", &ctx, &device)) return -1;
     Host* h = reinterpret_cast<Host*>(self);
     h->ctx = reinterpret_cast<ltca_ctx*>(static_cast<uintptr_t>(ctx));
     h->device = device;
-    h->stream = reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream));
     if (!h->ws) h->ws = new at::Tensor();
     return 0;
 }
@@ -729,7 +733,7 @@ PyMODINIT_FUNC PyInit__host(void) {
     HostType.tp_name = "cuda_ltc_b200._host.Host";
     HostType.tp_basicsize = sizeof(Host);
     HostType.tp_flags = Py_TPFLAGS_DEFAULT;
-    HostType.tp_doc = "Calls of one ltca_ctx: Host(context address, device, stream address).";
+    HostType.tp_doc = "Calls of one ltca_ctx: Host(context address, device).";
     HostType.tp_new = PyType_GenericNew;
     HostType.tp_init = host_init;
     HostType.tp_dealloc = host_dealloc;

@@ -132,6 +132,8 @@ int ltca_ctx_create(int device, void* stream, ltca_ctx** out);
  * may be placed on the GPU and set up its barriers while the kernel before it in the stream (this library's or the
  * caller's) is still running, but it touches no memory before that kernel has completed. */
 int ltca_ctx_set_stream(ltca_ctx* ctx, void* stream);
+/* The stream that the context's calls enqueue on: what ltca_ctx_create or the last ltca_ctx_set_stream was given. */
+int ltca_ctx_get_stream(const ltca_ctx* ctx, void** stream_out);
 void ltca_ctx_destroy(ltca_ctx* ctx);
 /* Text of the last error on this context (host string, valid until the next call). */
 const char* ltca_last_error(const ltca_ctx* ctx);
