@@ -78,6 +78,15 @@ class Context:
         except Exception:
             pass
 
+    def stream(self) -> torch.cuda.Stream:
+        """The stream that the calls enqueue on."""
+        at = C.c_void_p()
+        self.check(self.lib.ltca_ctx_get_stream(self.handle, C.byref(at)))
+        for s in (torch.cuda.current_stream(self.device), torch.cuda.default_stream(self.device)):
+            if s.cuda_stream == (at.value or 0):
+                return s
+        return torch.cuda.ExternalStream(at.value, device=self.device)
+
     def set_stream(self, stream: torch.cuda.Stream):
         self.lib.ltca_ctx_set_stream(self.handle, C.c_void_p(stream.cuda_stream))
 
@@ -200,9 +209,16 @@ class Context:
         """An empty cache for B sequences of up to ``capacity`` tokens; ``bounds=True`` for one that kv8_select is called on."""
         dev = torch.device("cuda", self.device)
         nb = -(-capacity // block)
-        k, v = (torch.zeros((B, H, capacity, D), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
-        ks, vs = (torch.ones((B, H, nb), dtype=torch.float32, device=dev) for _ in range(2))
-        return Kv8Cache(k, v, ks, vs, torch.zeros((B, H, nb, 2, D), dtype=torch.int8, device=dev) if bounds else None, block)
+        # filled in the order of the stream that the calls on it come in, and the current stream's to use as well
+        now, own = torch.cuda.current_stream(dev), self.stream()
+        with torch.cuda.stream(own):
+            k, v = (torch.zeros((B, H, capacity, D), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
+            ks, vs = (torch.ones((B, H, nb), dtype=torch.float32, device=dev) for _ in range(2))
+            ends = torch.zeros((B, H, nb, 2, D), dtype=torch.int8, device=dev) if bounds else None
+        if own.cuda_stream != now.cuda_stream:
+            for t in (k, v, ks, vs, *([ends] if bounds else [])):
+                t.record_stream(now)
+        return Kv8Cache(k, v, ks, vs, ends, block)
 
     def kv8_append(self, cache, k, v, kv_len, new_len=None):
         """Quantises new keys and values [B, H, n, D] into the cache at positions kv_len - new_len on, where ``kv_len`` (int32

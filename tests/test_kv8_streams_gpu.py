@@ -5,6 +5,7 @@ import torch
 
 import cuda_ltc_b200 as ltc
 from test_kv8_gpu import device_cache, filled, ints, queries
+from util import randn
 
 pytestmark = pytest.mark.gpu
 
@@ -90,6 +91,24 @@ def test_results_and_scratch_in_a_captured_graph(given, aside):
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and all((t == 7).all().item() for t in others)
 
 
+@pytest.mark.parametrize("bounds", [False, True])
+def test_a_new_cache_is_written_behind_its_making(aside, bounds):
+    """The current stream is busy when the cache is made: what is appended right after stays."""
+    c, stream = aside
+    k, v = (torch.from_numpy(randn((2, 2, 70, 64), i)).cuda().bfloat16() for i in range(2))
+    n = ints([70, 33])
+    want = c.kv8_cache(2, 2, 70, 64, bounds=bounds)
+    c.kv8_append(want, k, v, n)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        busy(torch.cuda.current_stream())
+        cache = c.kv8_cache(2, 2, 70, 64, bounds=bounds)
+        c.kv8_append(cache, k, v, n)
+        torch.cuda.synchronize()
+        for a, b in zip(cache[:5], want[:5]):
+            assert a is b is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_the_stream_is_the_contexts_own_whoever_sets_it(aside):
     import ctypes as C
     c, stream = aside
@@ -97,4 +116,5 @@ def test_the_stream_is_the_contexts_own_whoever_sets_it(aside):
     for s in (stream, torch.cuda.Stream(), torch.cuda.current_stream()):
         c.lib.ltca_ctx_set_stream(c.handle, C.c_void_p(s.cuda_stream))
         assert c.lib.ltca_ctx_get_stream(c.handle, C.byref(at)) == 0 and (at.value or 0) == s.cuda_stream
+        assert c.stream().cuda_stream == s.cuda_stream
     assert c.lib.ltca_ctx_get_stream(None, C.byref(at)) == -1 and c.lib.ltca_ctx_get_stream(c.handle, None) == -1
