@@ -730,6 +730,16 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
             return top > kLimit;
         };
         if (__builtin_expect(__any_sync(0xffffffffu, weigh()), 0)) {
+            // The scores as fp32 has them, and no longer products behind which the reference lies by up to half a unit in their last
+            // place: from 2^28 on that would be a weight above fp16's range.
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[g][t][x] *= ck[g][t][x & 1];
+                    ck[g][t][0] = ck[g][t][1] = 1.f;
+                }
             float lv[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) lv[g] = fmaxf(log2f(v_scale[g]), -110.f);
@@ -740,7 +750,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                     float top[NG];
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        top[g] = fmaxf(s[g][t][x] * ck[g][t][x], s[g][t][x + 2] * ck[g][t][x]);
+                        top[g] = fmaxf(s[g][t][x], s[g][t][x + 2]);
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) top[g] = fmaxf(top[g], __shfl_xor_sync(0xffffffffu, top[g], off));
                     }
