@@ -16,11 +16,16 @@
 // into a ring of the warp's own (a lane issues a step's copies; full bandwidth wants some 130 KB on their way to an SM, and with
 // cp.async the warps stood in line to issue them).
 //
-// Softmax.  With t the score in powers of two, a row keeps a reference m and e (whole numbers) and
-//     l = sum 2^(t - m),      O = sum 2^(t - m) (v_scale 2^(6 - e)) code.
-// e makes room for values of any size in fp16's range: weights lie around 2^6 where they matter, are as fine as 2^-24, and may
-// rise to 2^14 before m and e have to move.  So the usual step asks one vote of the warp instead of a reduction of maxima and
-// a multiplication of O, and every factor that ever touches O is a power of two.
+// Softmax.  With t the score in powers of two, a row keeps a reference m (a whole number) and
+//     l = sum 2^(t - m),      O = sum 2^(t - m) v_scale code.
+// A weight has to go through fp16, which has 11 bits down to 2^-14, 2^-24 at the least and 2^16 at the most.
+//   - bf16 rows: the products are summed on the tensor pipe, so that the scale of the values has to go with the weight.  A second
+//     whole number e takes it out again, 2^(t - m) (v_scale 2^(6 - e)): weights lie around 2^6 where they matter and may rise to
+//     2^14 before m and e have to move.  What weighs a row's largest weight times scale by 2^-20 and less loses bits, 2^-31 is lost.
+//   - fp32 rows: each product is added by the FMA pipe, which multiplies by the scale on the way; weights are 2^(t - m + 10), of two
+//     terms, with 22 bits down to 2^-13 of the largest, and 2^-35 at the least.
+// So the usual step asks one vote of the warp instead of a reduction of maxima and a multiplication of O, and every factor that
+// ever touches O is a power of two.
 //
 // Every warp works for itself.  The steps of all units (a pair and up to 8 NT of its rows) lie in one line, each unit's behind
 // a blank that stands for what a unit costs beside them, and a warp takes an equal run of it, whatever the lengths; it fetches
@@ -53,6 +58,9 @@ constexpr int kUnitCost = 3;                // what a unit costs beside its step
 constexpr int kNowhere = 0x7fffffff;        // the position of a group that is not there
 constexpr float kNone = -3.402823466e38f;   // the reference of a row that has seen no key
 constexpr float kLimit = 16384.f;           // largest weight before the references move
+// With fp32 rows: what a weight is multiplied by, and the scale of its values, so that O is 2^-24 of what it stands for and sums of
+// values near the end of fp32's range stay inside (e is then 30, a constant).
+constexpr float kWeight = 0x1p10f, kValue = 0x1p-34f, kFixed = 30.f;
 
 // A warp's ring: its steps are SG groups of 16 keys, 4 to 8 KB, and all but one are in flight.
 constexpr int step_groups(int D) { return D == 32 ? 4 : 2; }
@@ -114,9 +122,10 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 // a long sequence comes to 1e-6 of the result; with fp32 rows every product is therefore summed from zero and added by the FMA
 // pipe, to nearest (8 sequences of up to 16384 keys against 64 bits: 1.4e-6 without, 3.3e-7 with, for 5 to 9 % of the time with up to
 // eight rows and up to 30 % with sixteen).
+// `by`: a factor of the product (with two terms only).
 template <int kTerms>
 __device__ __forceinline__ void add_product(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b0)[kTerms],
-                                            const uint32_t (&b1)[kTerms]) {
+                                            const uint32_t (&b1)[kTerms], float by = 1.f) {
     if constexpr (kTerms == 1) {
         mma(d, a0, a1, a2, a3, b0[0], b1[0]);
     } else {
@@ -124,7 +133,7 @@ __device__ __forceinline__ void add_product(float (&d)[4], uint32_t a0, uint32_t
 #pragma unroll
         for (int i = kTerms - 1; i >= 0; --i) mma(x, a0, a1, a2, a3, b0[i], b1[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] += x[i];
+        for (int i = 0; i < 4; ++i) d[i] = fmaf(x[i], by, d[i]);
     }
 }
 // An 8 x 8 matrix of 16-bit values, two of a row in each lane, transposed.
@@ -498,6 +507,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 
     // ---- a unit's rows: 2c and 2c + 1 of each tile of 8 are this lane's in S^T and O^T, row r in Q ----
     float m[NT][2], inv[NT][2], e[NT][2], l[NT][2], cs[NT][2];       // inv = 2^(6 - e); cs: what a row's S is multiplied by
+    // (with two terms e stays at kFixed and inv is not used)
     int lim[NT][2];                                               // keys below it are seen
     int lim_min = 0;
     float o[NT][W][4];
@@ -508,7 +518,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) { m[t][k] = kNone; e[t][k] = 200.f; inv[t][k] = pow2(-100); l[t][k] = 0.f; }
+            for (int k = 0; k < 2; ++k) { m[t][k] = kNone; e[t][k] = kTerms == 2 ? kFixed : 200.f; inv[t][k] = pow2(-100); l[t][k] = 0.f; }
 #pragma unroll
             for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -609,7 +619,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
             // a group that is not there has whatever the ring held: all of it is hidden, and its scales are not looked at
             const bool there = pos[g] != kNowhere;
             k_scale[g] = there ? sc.x : 1.f;
-            v_scale[g] = there ? sc.y : 1.f;
+            v_scale[g] = there ? (kTerms == 2 ? fminf(sc.y * kValue, 1e38f) : sc.y) : 1.f;
             some |= there;
             whole &= pos[g] <= lim_min - 16;
         }
@@ -711,27 +721,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
 #pragma unroll
                 for (int t = 0; t < NT; ++t) ck[g][t][0] = ck[g][t][1] = 1.f;
         }
-        float p[NG][NT][4], w[NG][NT][4];
-        auto weigh = [&]() -> bool {
-            float top = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    // between bounds that no weight which counts comes near, so that 0 * f is 0 and a large p shows in w
-                    const float f[2] = {fmaxf(fminf(v_scale[g] * inv[t][0], 1e38f), 1e-24f), fmaxf(fminf(v_scale[g] * inv[t][1], 1e38f), 1e-24f)};
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        p[g][t][x] = exp2_fast(fmaf(s[g][t][x], ck[g][t][x & 1], -m[t][x & 1]));
-                        w[g][t][x] = p[g][t][x] * f[x & 1];
-                        top = fmaxf(top, w[g][t][x]);
-                    }
-                }
-            return top > kLimit;
-        };
-        if (__builtin_expect(__any_sync(0xffffffffu, weigh()), 0)) {
-            // The scores as fp32 has them, and no longer products behind which the reference lies by up to half a unit in their last
-            // place: from 2^28 on that would be a weight above fp16's range.
+        auto scale_scores = [&]() {
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -740,38 +730,116 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                     for (int x = 0; x < 4; ++x) s[g][t][x] *= ck[g][t][x & 1];
                     ck[g][t][0] = ck[g][t][1] = 1.f;
                 }
-            float lv[NG];
+        };
+        if constexpr (kTerms == 2) scale_scores();                // (frees registers, which these builds lack: 217 us for 208)
+        float p[NG][NT][4], w[NG][NT][4];
+        auto weigh = [&]() -> bool {
+            float top = 0.f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) lv[g] = fmaxf(log2f(v_scale[g]), -110.f);
+            for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
+                    float f[2] = {kWeight, kWeight};
+                    if constexpr (kTerms == 1) {
+                        // between bounds that no weight which counts comes near, so that 0 * f is 0 and a large p shows in w
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    float top[NG];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        top[g] = fmaxf(s[g][t][x], s[g][t][x + 2]);
-#pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) top[g] = fmaxf(top[g], __shfl_xor_sync(0xffffffffu, top[g], off));
+                        for (int x = 0; x < 2; ++x) f[x] = fmaxf(fminf(v_scale[g] * inv[t][x], 1e38f), 1e-24f);
                     }
-                    float m2 = m[t][x];
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) m2 = fmaxf(m2, ceilf(top[g]));
-                    const float before = m[t][x] == kNone ? -INFINITY : e[t][x] + (m[t][x] - m2);
-                    float y = before;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) y = fmaxf(y, ceilf(top[g] - m2 + lv[g]));
-                    if (y > -1000.f && y < 1000.f) {              // a row that has seen a key
-                        const float fo = before == -INFINITY ? 1.f : exp2_fast(before - y);
-                        l[t][x] *= m[t][x] == kNone ? 1.f : exp2_fast(m[t][x] - m2);
-                        m[t][x] = m2;
-                        e[t][x] = y;
-                        inv[t][x] = exp2_fast(6.f - y);
-#pragma unroll
-                        for (int i = 0; i < W; ++i) { o[t][i][x] *= fo; o[t][i][x + 2] *= fo; }
+                    for (int x = 0; x < 4; ++x) {
+                        p[g][t][x] = exp2_fast(fmaf(s[g][t][x], ck[g][t][x & 1], -m[t][x & 1]));
+                        w[g][t][x] = p[g][t][x] * f[x & 1];
+                        if constexpr (kTerms == 2) p[g][t][x] = w[g][t][x];      // (l is brought down once, where it leaves)
+                        top = fmaxf(top, w[g][t][x]);
                     }
                 }
+            return top > kLimit;
+        };
+        if (__builtin_expect(__any_sync(0xffffffffu, weigh()), 0)) {
+            // The scores as fp32 has them, and no longer products behind which the reference lies by up to half a unit in their last
+            // place: from 2^28 on that would be a weight above fp16's range.
+            scale_scores();
+            // `worth`: what the weight of key r, or r + 8, brings to O besides itself, in powers of two
+            auto move = [&](const float (&worth)[NG][2]) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) top = fmaxf(top, fmaxf(s[g][t][x], s[g][t][x + 2]));
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                        const float m2 = fmaxf(m[t][x], ceilf(top));
+                        const bool first = m[t][x] == kNone;
+                        const float dm = m[t][x] - m2;
+                        float y = e[t][x], fo = 1.f;
+                        bool moves = m2 > kNone && m2 < INFINITY;    // the row has seen a key
+                        if constexpr (kTerms == 1) {
+                            y = -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) y = fmaxf(y, fmaxf(s[g][t][x] - m2 + worth[g][0], s[g][t][x + 2] - m2 + worth[g][1]));
+#pragma unroll
+                            for (int off = 4; off < 32; off <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off));
+                            y = fmaxf(first ? -INFINITY : e[t][x] + dm, ceilf(y));
+                            moves = y > -1000.f && y < 1000.f;
+                        }
+                        if (moves) {
+                            if (!first) fo = exp2_fast(kTerms == 1 ? e[t][x] + dm - y : dm);
+                            l[t][x] *= first ? 1.f : exp2_fast(dm);
+                            m[t][x] = m2;
+                            if constexpr (kTerms == 1) { e[t][x] = y; inv[t][x] = exp2_fast(6.f - y); }
+#pragma unroll
+                            for (int i = 0; i < W; ++i) { o[t][i][x] *= fo; o[t][i][x + 2] *= fo; }
+                        }
+                    }
+            };
+            float worth[NG][2];
+            uint32_t zero = 0;                                      // keys that have no value but zero: bit 2 g, 2 g + 1
+            if constexpr (kTerms == 1) {
+                // A weight brings itself times the scale of its values - unless they are all zero, when a reference by the scale
+                // could push what the others bring out of fp16.  Keys with four zeros are looked at whole.
+                bool some_zero = false;
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        worth[g][x] = fmaxf(log2f(v_scale[g]), -110.f);
+                        some_zero |= (*reinterpret_cast<const uint32_t*>(body + (SG + g) * Gr::kBytes + x * 8 * D + k_at) & 0x7f7f7f7fu) == 0;
+                    }
+                if (__builtin_expect(__any_sync(0xffffffffu, some_zero), 0)) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t any = 0;
+#pragma unroll
+                            for (int part = 0; part < Gr::kParts; ++part) {
+                                const uint32_t* src = reinterpret_cast<const uint32_t*>(body + (SG + g) * Gr::kBytes + x * 8 * D + (k_at ^ part * 64));
+#pragma unroll
+                                for (int i = 0; i < Gr::kWords; ++i) any |= src[i] & 0x7f7f7f7fu;
+                            }
+                            any |= __shfl_xor_sync(0xffffffffu, any, 1);
+                            any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                            if (any == 0) {
+                                zero |= 1u << (2 * g + x);
+                                worth[g][x] = -110.f;               // as the smallest value there is
+                            }
+                        }
+                }
+            }
+            move(worth);
             weigh();
+            if constexpr (kTerms == 1)
+                if (__builtin_expect(zero != 0, 0)) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                if (zero >> (2 * g + (x >> 1)) & 1) w[g][t][x] = 0.f;
+                }
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -852,7 +920,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 codes_to_half2(__byte_perm(v[0][i >> 1], v[1][i >> 1], sel), a0, a1);
                 codes_to_half2(__byte_perm(v[2][i >> 1], v[3][i >> 1], sel), a2, a3);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) add_product<kTerms>(o[t][i], a0, a1, a2, a3, w0[t], w1[t]);
+                for (int t = 0; t < NT; ++t) add_product<kTerms>(o[t][i], a0, a1, a2, a3, w0[t], w1[t], v_scale[g]);
             }
         }
     };
@@ -871,6 +939,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                 float sum = l[t][x];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                if constexpr (kTerms == 2) sum *= 1.f / kWeight;
                 const int row = t * 8 + 2 * c + x;
                 if (mine) {
                     T* out = reinterpret_cast<T*>(a.p.o) + __shfl_sync(0xffffffffu, place, row) + r * (D / 8);

@@ -282,8 +282,11 @@ int ltca_kv8_read(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_read_pa
  * Attention of the newest tokens over the cache: O = softmax(mask(scale * Q K^T)) V.  Heads of queries may share a head of
  * keys: head h reads head h / (Hq/H).  Query i of sequence b stands at position kv_len[b] - new_len[b] + i; rows from
  * new_len[b] on, and rows that see no key, give zeros and lse = -inf.  Scores and statistics are fp32; products run on the
- * tensor pipe with the codes as they are (e4m3 is exact in fp16) and Q and P in fp16, for fp32 queries in two fp16 terms each
- * (22 bits).  A few tens of rows (new tokens x heads that share) per head of keys are what the kernel is made for; long
+ * tensor pipe with the codes as they are (e4m3 is exact in fp16) and Q and P in fp16, for fp32 queries in two fp16 terms each.
+ * Q is held to 2^-25 of its row's largest element at the least (bf16 queries: exactly, down to 2^-17 of it).  P has, with bf16
+ * queries, 11 bits down to 2^-20 of the row's largest weight times scale of its values (keys whose values are all zero left aside)
+ * and nothing below 2^-31 of it; with fp32 queries 22 bits down to 2^-13 of the largest weight and nothing below 2^-35.
+ * A few tens of rows (new tokens x heads that share) per head of keys are what the kernel is made for; long
  * chunks of a prompt are faster through ltca_kv8_read and ltca_attn_fwd.
  */
 typedef struct {
