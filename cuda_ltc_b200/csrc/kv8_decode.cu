@@ -51,7 +51,7 @@ namespace {
 constexpr int kWarps = 4;                   // of a CTA
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHead = 48;                   // a step's positions and scales
-constexpr int kMaxCluster = 8;              // CTAs that join their shares through shared memory
+constexpr int kMaxCluster = 8;              // CTAs that join their shares through shared memory (more would be a launch's opt-in)
 constexpr int kClusterSteps = 8;            // of a warp there, at most
 constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do
 constexpr int kUnitCost = 3;                // what a unit costs beside its steps, in steps
@@ -1232,14 +1232,6 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.splits > 1 ? 2 : 1;
-    if (a.splits > 8) {
-        static SmemOptIn wide;      // clusters of more than eight CTAs are an opt-in of a kernel on one device
-        const uint64_t bit = (ctx->device >= 0 && ctx->device < 64) ? (1ull << ctx->device) : 0ull;
-        if (!bit || !(wide.done.load(std::memory_order_acquire) & bit)) {
-            LTCA_CUDA_OK(ctx, cudaFuncSetAttribute(kv8_decode_kernel<T, D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            wide.done.fetch_or(bit, std::memory_order_release);
-        }
-    }
     LTCA_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kv8_decode_kernel<T, D, NT>, a, k_map, v_map));
     return LTCA_OK;
 }
