@@ -15,4 +15,4 @@ def test_wide_clusters_are_opted_into_where_they_occur():
         if largest:
             seen[name] = max(largest)
             assert ("cudaFuncAttributeNonPortableClusterSizeAllowed" in text) == (max(largest) > 8), name
-    assert seen == {"kv8_decode.cu": 8, "kv8_select.cu": 16}
+    assert seen == {"attn_decode.cu": 16, "kv8_decode.cu": 8, "kv8_select.cu": 16}
