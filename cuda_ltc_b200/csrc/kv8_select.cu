@@ -42,7 +42,9 @@ __device__ __forceinline__ uint32_t signs(uint32_t x) {
 constexpr int kThreads = 256, kSelectWarps = kThreads / 32;
 constexpr int kRowsAtATime = 32;            // rows of Q in shared memory
 constexpr int kMaxSelectCluster = 16;
-constexpr int kGather = 16384;              // blocks whose scores one CTA goes through
+constexpr int kGather = 4096;             // blocks whose scores one CTA goes through; from there on its rounds take longer than the cluster's
+                                          // barriers (one sequence, 8 heads of 128: 2048 blocks 10.8 us, with the cluster 13.3; 8192 35.7 and 21.6,
+                                          // 16384 69.9 and 35.6; eight sequences 2048 24.1 and 30.0, 4096 41.6 and 43.9, 8192 82.9 and 70.7)
 constexpr int kAtOnce = 4;                  // blocks of a lane whose bounds are on their way together
 
 template <typename T, int D, bool kGathered>
