@@ -13,8 +13,8 @@
 //
 // The order of the contracted index is free as long as both operands agree.  A lane therefore takes whole pieces of rows: of
 // K, D/4 bytes of two keys; of V, D/8 bytes of four keys, whose bytes a permutation brings side by side.  The rows come by TMA
-// into a ring of the warp's own (a lane issues a step's copies; full bandwidth wants some 130 KB on their way to an SM, and with
-// cp.async the warps stood in line to issue them).
+// into a ring of the warp's own (a lane issues a step's copies; with cp.async the warps stood in line to issue them), all of whose steps but
+// one are on their way: 96 KB of an SM with heads of 128 and 128 KB with narrower ones, up to eight rows, and 64 to 96 KB with sixteen.
 //
 // Softmax.  With t the score in powers of two, a row keeps a reference m (a whole number) and
 //     l = sum 2^(t - m),      O = sum 2^(t - m) v_scale code.
@@ -32,13 +32,16 @@
 // across the borders of units, so that the stream does not stop while a unit's queries are brought in or its sums leave.  A
 // unit that one warp has seen whole is finished by it; shares of a unit go to scratch and are joined by a second kernel.
 // Calls that are over in a few steps take no line: the CTAs of a cluster divide a unit's steps and join their shares through
-// each other's shared memory, in one launch (3 sequences of up to 4000 keys 10.6 us, on the line 17).
+// each other's shared memory, in one launch (3 sequences of up to 4000 keys 11.0 us; on the line, at an earlier step, 17 against 10.6).
 //
-// Measured: 74 sequences of 8192 keys of 128, 8 heads of keys, 1 / 8 / 16 rows each: 206 / 208 / 241 us = 6.0 / 6.0 / 5.2 TB/s;
-// 16384 keys of 64: 212 / 214 / 281 us; fp32 rows 215 / 220 / 370 and 254 / 255 / 410.  Long streams of up to eight rows are bound by
-// memory, with sixteen by the waits of the few warps that the registers leave on an SM (instructions 40 % of the issue slots).
-// Many short sequences pay for what a unit costs beside its steps, about 3500 cycles, and for the join: 256 of up to 1024 keys
-// of 64 run at 42 us, twice the memory's time.
+// Measured: 74 full caches, 8 heads of keys, 1 / 8 / 16 rows each, bf16 rows and fp32 rows (1.24 GB, 193 us at the memory's rate):
+//     8192 keys of 128     204 / 207 / 235 us    208 / 211 / 333
+//     16384 keys of 64     216 / 218 / 298       254 / 256 / 394
+//     32768 keys of 32     261 / 262 / 360       308 / 310 / 478
+// Up to eight rows of 128 are bound by memory.  Sixteen rows are bound by the waits of the few warps that the registers leave on an SM
+// (fp32 at 64 also spills), and narrow heads by the work per key, which does not shrink with a key's bytes.  Many short sequences pay
+// for what a unit costs beside its steps (by stamps of an earlier step 3500 cycles, with sixteen rows 17000) and for the join: 256 of up to 1024 keys of 64, fp32 rows 47.5 us,
+// bf16 rows 41.7, twice the memory's time of 21.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
@@ -52,9 +55,13 @@ constexpr int kWarps = 4;                   // of a CTA
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHead = 48;                   // a step's positions and scales
 constexpr int kMaxCluster = 8;              // CTAs that join their shares through shared memory (more would be a launch's opt-in)
-constexpr int kClusterSteps = 8;            // of a warp there, at most
-constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do
-constexpr int kUnitCost = 3;                // what a unit costs beside its steps, in steps
+constexpr int kClusterSteps = 8;            // of a warp there, at most (8 rows of 128: 8000 keys 16.6 us with 4, 17.6 with 8; 16000 keys 19.3 with 8,
+                                            // 26.9 with 16; 128 pairs of up to 3000 keys 22.9 with 4, 21.7 with 8)
+constexpr int kMinCost = 4;                 // of a warp's run, where there is little to do (600 pairs of 64 keys of 64: 13.2 us with 2, 13.5 with 4, 17.2 with
+                                            // 8; 8 of 16000 keys of 128: 20.7, 19.3, 21.2)
+// What a unit costs beside its steps, in steps (1 / 3 / 5: 256 sequences of up to 1024 keys of 64, bf16 54.1 / 42.4 / 43.0 us, fp32 57.4 / 48.3 / 50.9;
+// 16 rows, 32 sequences of up to 6001 keys of 128 68.8 / 57.1 / 55.9, 75 of up to 1024 54.9 / 44.8 / 44.1: nearer five there).
+constexpr int kUnitCost = 3;
 constexpr int kNowhere = 0x7fffffff;        // the position of a group that is not there
 constexpr float kNone = -3.402823466e38f;   // the reference of a row that has seen no key
 constexpr float kLimit = 16384.f;           // largest weight before the references move
@@ -68,8 +75,8 @@ template <int D> constexpr int kGroups = step_groups(D);
 template <int D> constexpr int kStepBytes = kGroups<D> * 32 * D;
 template <int D> constexpr int kStages = D == 128 ? 2 : 3;
 // CTAs of an SM, by the registers that NT tiles of 8 rows take
-// (four of 64 channels: 128 registers a thread and three stages; with three CTAs of four stages fp32 rows took 238 us for 220,
-// 256 short sequences 49.6 for 42.9, bf16 rows of long ones 211 for 221)
+// (four of 64 channels: 128 registers a thread and three stages; with three CTAs of four stages 74 long caches took 228 us for 209, 256 short
+// sequences 46.6 for 42.4 with bf16 rows and 49.7 for 48.3 with fp32)
 constexpr int ctas_per_sm(int D, int nt) { return nt * D >= 256 ? 2 : nt == 1 && D <= 64 ? 4 : 3; }
 template <int D, int NT> constexpr int kCtas = ctas_per_sm(D, NT);
 constexpr int kLens = 256;                  // lengths in shared memory
@@ -731,7 +738,7 @@ kv8_decode_kernel(const __grid_constant__ DecodeArgs a, const __grid_constant__ 
                     ck[g][t][0] = ck[g][t][1] = 1.f;
                 }
         };
-        if constexpr (kTerms == 2) scale_scores();                // (frees registers, which these builds lack: 217 us for 208)
+        if constexpr (kTerms == 2) scale_scores();                // (frees registers, which these builds lack: 230 us for 208 at 74 caches of 8192 keys of 128)
         float p[NG][NT][4], w[NG][NT][4];
         auto weigh = [&]() -> bool {
             float top = 0.f;
@@ -1209,7 +1216,9 @@ int launch(ltca_ctx* ctx, const DecodeArgs& a) {
     if (!a.splits) {
         const dim3 grid((unsigned)((a.warps + kWarps - 1) / kWarps));
         LTCA_CUDA_OK(ctx, launch_dependent(kv8_decode_kernel<T, D, NT>, grid, dim3(kThreads), bytes, ctx->stream, a, k_map, v_map));
-        // a CTA for each row where a unit has many shares
+        // a CTA for each row where a unit has many shares (8 rows of 16000 / 30000 keys of 128, 74 and more warps a unit: 19.3 / 25.0 us, with a
+        // warp a row 43.0 / 65.8; 4 warps a unit 209 and 211; between 9 and 14 a CTA a row is faster for one row and for four, 23.9 against 28.4
+        // and 30.8 against 32.8, and slower for eight, 106.0 against 102.8)
         const bool wide = a.warps > 16 * units;
         auto join = wide ? kv8_decode_join_kernel<T, D, true> : kv8_decode_join_kernel<T, D, false>;
         const int64_t rows = units * a.rows;

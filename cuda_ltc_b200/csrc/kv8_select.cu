@@ -6,10 +6,10 @@
 //   - The `count` best: the score's bits in an order that whole numbers have, and a search for the count-th largest of them
 //     eight bits at a time with histograms in shared memory.  Up to kGather blocks the scores go to the cluster's first CTA,
 //     which searches alone, from the highest bit in which they differ on: two or three rounds.  With more blocks every CTA keeps
-//     its own, and the cluster adds up the histograms, at about 1.2 us a round (8 pairs' worth of 2048 blocks: 16.4 us in all).
+//     its own, and the cluster adds up the histograms (times of both at kGather).
 //   - The indices come out in rising order, since it is known how many of the blocks before have been taken.
 // Bound by the waits one behind another - lengths, queries, bounds, the cluster, the search - of about a microsecond each: 2048
-// blocks of 8 sequences and 8 heads 15 us, of which the bounds (2 D + 4 bytes a block) take 3.8; 256 blocks of one sequence 6 us.
+// blocks of 8 sequences and 8 heads 15 us, of which the bounds (2 D + 4 bytes a block) take 3.8; 256 blocks of one sequence 6 us; 4096 of eight 42 us, 16384 124 us.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
@@ -387,7 +387,8 @@ int launch_blocks(ltca_ctx* ctx, const SelectArgs& a) {
 
 int launch_kv8_select(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_select_params* p) {
     SelectArgs a{*c, *p, (c->S + c->block - 1) / c->block, p->Hq / c->H, p->Hq / c->H * p->Sq, 1, 0};
-    // about two CTAs per SM, each with 64 blocks at least
+    // About two CTAs per SM, each with 64 blocks at least.  Both sides, 8 heads of 128, 32 / 64 / 128 at least: one sequence of 256 blocks 5.7 /
+    // 6.4 / 7.4 us, eight of 256 9.4 / 7.1 / 7.8, eight of 512 11.5 / 11.5 / 9.0; with 1024 blocks and more all three are alike.
     const int64_t pairs = (int64_t)c->B * c->H;
     while (a.ctas < kMaxSelectCluster && pairs * a.ctas < 2 * kPlanSms && a.nb / (2 * a.ctas) >= 64) a.ctas *= 2;
     while (a.ctas < kMaxSelectCluster && (a.nb + a.ctas - 1) / a.ctas > 48 * 1024) a.ctas *= 2;

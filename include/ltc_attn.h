@@ -312,7 +312,9 @@ typedef struct {
     size_t workspace_bytes;
 } ltca_kv8_decode_params;
 int ltca_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decode_params* p);
-/* Room for the shares of rows that several warps work on: 5 to 20 MB for large calls, little for small ones. */
+/* Room for the shares of rows that several warps work on.  None where clusters take the call; else W R (D + 4) 8 bytes for W warps
+ * (at most 1184 to 2368, by D and rows) and R rows of a tile (at most 16), and 8 more for each head of keys and 16 rows of it: for
+ * large calls 0.7 MB (one row of 32) to 20 MB (16 rows of 128), and the table. */
 int ltca_kv8_decode_workspace_bytes(const ltca_kv8_cache* c, const ltca_kv8_decode_params* p, size_t* bytes_out);
 
 /*
@@ -320,8 +322,9 @@ int ltca_kv8_decode_workspace_bytes(const ltca_kv8_cache* c, const ltca_kv8_deco
  * and a head of queries) is rounded to eight bits with a power-of-two step, the smallest from 2^-100 on by which its largest
  * finite magnitude comes down to 127; a block's score is the largest over the rows of
  *     sum_d max(q_d lo_d, q_d hi_d) * k_scale * step       (lo, hi: the block's bounds)
- * which no product of that row with one of the block's keys exceeds by more than the rounding of Q; the sum is one of whole
- * numbers, so that the choice does not depend on an order of additions.  NaN in Q counts as zero, an infinity as +-127.  The `first` blocks and the `last` live ones are
+ * of which four times - lo and hi are quarters of codes - no product of that row with one of the block's keys exceeds by more than
+ * the rounding of Q; the sum is one of whole numbers, so that the choice does not depend on an order of additions.  NaN in Q counts as
+ * zero, an infinity as +-127.  The `first` blocks and the `last` live ones are
  * always taken; equal scores go to the lower index.  blocks: the indices in rising order, then -1 where a sequence has fewer.
  */
 typedef struct {

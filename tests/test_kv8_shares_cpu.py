@@ -43,3 +43,59 @@ def test_the_join_asks_before_it_forms_an_address():
     read, asked = join.index("a.shares["), join.index("shares_are_there(who.x, who.y, a.warps)")
     used = [m.start() for m in re.finditer(r"who\.[xy]", join) if not asked <= m.start() <= asked + 60]
     assert read < asked < min(used)
+
+
+def _workspace(B, H, G, Sq, S, D, dtype, n_blocks=0):
+    import ctypes as C
+    from cuda_ltc_b200 import _lib
+    c = _lib.Kv8CacheParams(B=B, H=H, S=S, D=D, block=64)
+    p = _lib.Kv8DecodeParams(Hq=H * G, Sq=Sq, dtype=dtype, scale=1.0)
+    if n_blocks:
+        p.blocks, p.n_blocks = 256, n_blocks
+    n = C.c_size_t()
+    assert _lib.load().ltca_kv8_decode_workspace_bytes(C.byref(c), C.byref(p), C.byref(n)) == 0
+    return n.value
+
+
+def test_scratch_is_what_the_header_says():
+    """W R (D + 4) 8 bytes for at most W = 1184 .. 2368 warps and R rows of a tile, and 8 for each head of keys and tile of 8 or 16 rows;
+    both in pieces of 256."""
+    seen = []
+    for D in (32, 64, 128):
+        for rows in ((1, 1), (3, 2), (8, 1), (4, 4), (5, 7), (16, 64)):
+            for B, H, S in ((1, 1, 1), (1, 8, 100000), (300, 2, 64), (16, 8, 32768), (4096, 8, 1024), (1, 1, 1 << 30)):
+                for dtype in (0, 1):
+                    R = rows[0] * rows[1]
+                    n = _workspace(B, H, *rows, S, D, dtype)
+                    tiles = -(-R // (8 if R <= 8 else 16))
+                    warps = 1184 if R > 8 and D == 128 else 1776 if R > 8 or D == 128 else 2368
+                    most = warps * min(R, 8 if R <= 8 else 16) * (D + 4) * 8
+                    assert n <= most + 256 + B * H * tiles * 8 + 256, (D, rows, B, H, S, n)
+                    if S * B > 300000:
+                        assert n >= most, (D, rows, B, H, S, n)
+                    seen.append(n)
+    assert min(seen) == 0
+    assert 6.5e5 < _workspace(16, 8, 1, 1, 32768, 32, 1) < 7.5e5 and 2.0e7 < _workspace(16, 8, 16, 1, 32768, 128, 1) < 2.1e7
+
+
+def test_four_times_a_score_bounds_the_products():
+    """What the selection's score says of a block: its bounds are quarters of codes.  Blocks of different keys, whose bounds no single key
+    reaches, and one block of 16 equal keys along the query, which the score itself does not bound."""
+    import numpy as np
+    import kv8_ref
+    r = np.random.default_rng(0)
+    B, H, S, D, block = 1, 1, 320, 64, 16
+    ref = kv8_ref.Cache.empty(B, H, S, D, block)
+    k = r.standard_normal((B, H, S, D)).astype(np.float32)
+    q = r.standard_normal(D)
+    k[:, :, -block:] = q * 100
+    ref.append(k, k, [S])
+    step = 2.0 ** kv8_ref.pow2_down_to(q, 127.0, 121)
+    whole = np.round(q / step)
+    keys = ref.values()[0][0, 0].reshape(-1, block, D)
+    for j in range(S // block):
+        lo, hi = ref.bounds[0, 0, j].astype(float)
+        score = np.maximum(whole * lo, whole * hi).sum() * ref.ks[0, 0, j] * step
+        most, rounding = (keys[j] @ q).max(), 0.5 * step * np.abs(keys[j]).sum(1).max()
+        assert most <= 4 * score + rounding
+    assert most > score + rounding
