@@ -1,7 +1,7 @@
 // Writing keys and values into the 8-bit cache and reading them back: see ltca_kv8_cache in include/ltc_attn.h.
 // Both are bound by memory: each value is read once and written once.  Read: 8 sequences of up to 32768 keys of 128 to bf16
 // 205 us = 6.56 TB/s.  Append: prompts of up to 8000 tokens, 8 sequences of 8 heads of 128 with bounds 43 us = 4.56 TB/s, held
-// up by instructions (some 300 a thread for 64 values); a token of each of 256 sequences 2.6 us, a launch.
+// up by instructions (16 a value, 70 % of the issue slots); a token of each of 256 sequences 2.6 us, a launch.
 #include "kv8.cuh"
 
 namespace ltca {
