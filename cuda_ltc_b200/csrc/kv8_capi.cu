@@ -1,5 +1,7 @@
 // C-ABI entry points of the 8-bit key/value cache: argument checks in front of the kernels' launches.  Every index that a
 // kernel forms from these arguments and from what it reads on the device (lengths, block lists) is cut to the cache there.
+#include <initializer_list>
+
 #include "kv8.cuh"
 
 namespace ltca {
@@ -14,6 +16,18 @@ namespace {
 
 bool misaligned(const void* p, const ltca_strides& s, int to) {
     return reinterpret_cast<uintptr_t>(p) % to || s.batch % to || s.head % to || s.seq % to;
+}
+// Whether a pointer lies on a boundary of its elements: kernels read whole elements at the least.
+bool off_element(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size; }
+int check_words(ltca_ctx* ctx, std::initializer_list<const void*> words) {
+    for (const void* p : words)
+        if (off_element(p, 4)) return fail(ctx, LTCA_ERR_INVALID, "int32 and float32 arrays must be 4-byte aligned");
+    return LTCA_OK;
+}
+int check_elements(ltca_ctx* ctx, int dtype, std::initializer_list<const void*> tensors) {
+    for (const void* p : tensors)
+        if (off_element(p, elem_size(dtype))) return fail(ctx, LTCA_ERR_INVALID, "a tensor must be aligned to its elements (%d bytes)", elem_size(dtype));
+    return LTCA_OK;
 }
 // Whether two places of a [B,H,n,...] tensor share memory through a stride of zero.
 bool overlaps(const ltca_strides& s, int64_t B, int64_t H, int64_t n) {
@@ -37,7 +51,7 @@ int check_cache(ltca_ctx* ctx, const ltca_kv8_cache* c, bool k, bool v) {
     if ((k && misaligned(c->k, c->k_strides, 16)) || (v && misaligned(c->v, c->v_strides, 16)))
         return fail(ctx, LTCA_ERR_INVALID, "the cache's rows must start on 16-byte boundaries");
     if (reinterpret_cast<uintptr_t>(c->bounds) % 16) return fail(ctx, LTCA_ERR_INVALID, "bounds must be 16-byte aligned");
-    return LTCA_OK;
+    return check_words(ctx, {c->k_scale, c->v_scale});
 }
 int check_dtype(ltca_ctx* ctx, int dtype) {
     return dtype == LTCA_F32 || dtype == LTCA_BF16 ? LTCA_OK : fail(ctx, LTCA_ERR_INVALID, "bad dtype %d", dtype);
@@ -81,6 +95,8 @@ int ltca_kv8_append(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_appen
     if (p->n < 0) return fail(ctx, LTCA_ERR_INVALID, "negative number of tokens %d", p->n);
     if (p->n == 0) return LTCA_OK;
     if (!p->k || !p->v || !p->kv_len) return fail(ctx, LTCA_ERR_INVALID, "append needs k, v and kv_len");
+    if (int rc = check_elements(ctx, p->dtype, {p->k, p->v})) return rc;
+    if (int rc = check_words(ctx, {p->kv_len, p->new_len})) return rc;
     if (overlaps(c->k_strides, c->B, c->H, c->S) || overlaps(c->v_strides, c->B, c->H, c->S))
         return fail(ctx, LTCA_ERR_INVALID, "a cache that is written must not share memory between sequences, heads or tokens");
     OnDevice on(ctx->device);
@@ -97,6 +113,8 @@ int ltca_kv8_read(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_read_pa
         return fail(ctx, LTCA_ERR_INVALID, "bad range of positions %d + %d of %d", p->start, p->n, c->S);
     if (p->n == 0) return LTCA_OK;
     if (!p->k || !p->v) return fail(ctx, LTCA_ERR_INVALID, "null tensor");
+    if (int rc = check_elements(ctx, p->dtype, {p->k, p->v})) return rc;
+    if (int rc = check_words(ctx, {p->kv_len})) return rc;
     if (overlaps(p->k_strides, c->B, c->H, p->n) || overlaps(p->v_strides, c->B, c->H, p->n))
         return fail(ctx, LTCA_ERR_INVALID, "a result must not share memory between sequences, heads or tokens");
     OnDevice on(ctx->device);
@@ -118,6 +136,8 @@ int ltca_kv8_decode(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_decod
     if (int rc = check_cache(ctx, c, true, true)) return rc;
     if (int rc = check_queries(ctx, c, p->Hq, p->Sq, p->dtype, p->q)) return rc;
     if (!p->o) return fail(ctx, LTCA_ERR_INVALID, "null tensor");
+    if (int rc = check_elements(ctx, p->dtype, {p->q, p->o})) return rc;
+    if (int rc = check_words(ctx, {p->lse, p->keep_mask, p->kv_len, p->new_len, p->blocks})) return rc;
     if (!(p->scale > 0.f)) return fail(ctx, LTCA_ERR_INVALID, "scale must be positive");
     if (overlaps(p->o_strides, c->B, p->Hq, p->Sq))
         return fail(ctx, LTCA_ERR_INVALID, "a result must not share memory between sequences, heads or tokens");
@@ -136,6 +156,8 @@ int ltca_kv8_select(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_selec
     if (int rc = check_queries(ctx, c, p->Hq, p->Sq, p->dtype, p->q)) return rc;
     if (!c->bounds || !c->k_scale) return fail(ctx, LTCA_ERR_INVALID, "select needs a cache that keeps bounds");
     if (!p->blocks) return fail(ctx, LTCA_ERR_INVALID, "null tensor");
+    if (int rc = check_elements(ctx, p->dtype, {p->q})) return rc;
+    if (int rc = check_words(ctx, {p->kv_len, p->new_len, p->blocks})) return rc;
     if (p->count < 1 || p->first < 0 || p->last < 0 || (int64_t)p->first + p->last > p->count)
         return fail(ctx, LTCA_ERR_INVALID, "%d blocks with the first %d and the last %d among them", p->count, p->first, p->last);
     OnDevice on(ctx->device);

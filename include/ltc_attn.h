@@ -260,7 +260,7 @@ typedef struct {
 typedef struct {
     int32_t n;                  /* tokens of k and v; 0: nothing is done             */
     int32_t dtype;              /* ltca_dtype of k and v                             */
-    const void* k; ltca_strides k_strides;     /* [B,H,n,D], any alignment           */
+    const void* k; ltca_strides k_strides;     /* [B,H,n,D], rows on any element     */
     const void* v; ltca_strides v_strides;
     const int32_t* kv_len;      /* [B] length behind the call, not written           */
     const int32_t* new_len;     /* optional [B] (0 .. n): new tokens of a sequence; NULL: n */
@@ -274,7 +274,7 @@ int ltca_kv8_append(ltca_ctx* ctx, const ltca_kv8_cache* c, const ltca_kv8_appen
 typedef struct {
     int32_t start, n;           /* 0 <= start, start + n <= S; n = 0: nothing is done */
     int32_t dtype;              /* ltca_dtype of k and v                             */
-    void* k; ltca_strides k_strides;           /* [B,H,n,D], any alignment           */
+    void* k; ltca_strides k_strides;           /* [B,H,n,D], rows on any element     */
     void* v; ltca_strides v_strides;
     const int32_t* kv_len;      /* optional [B]; NULL: all S                         */
 } ltca_kv8_read_params;
@@ -299,8 +299,8 @@ typedef struct {
     int32_t causal;             /* key j visible to a query at position t iff j <= t */
     float   scale;              /* > 0                                               */
     float   score_clamp;        /* > 0: s = min(s, score_clamp) after scaling        */
-    const void* q; ltca_strides q_strides;     /* [B,Hq,Sq,D], any alignment         */
-    void*       o; ltca_strides o_strides;     /* [B,Hq,Sq,D], any alignment         */
+    const void* q; ltca_strides q_strides;     /* [B,Hq,Sq,D], rows on any element   */
+    void*       o; ltca_strides o_strides;     /* [B,Hq,Sq,D], rows on any element   */
     float*      lse;            /* optional [B,Hq,Sq]                                */
     const float*   keep_mask;   /* optional [B,Sq,S] contiguous; value 0 hides the key */
     const int32_t* kv_len;      /* optional [B], with the new tokens; NULL: all S    */
@@ -330,7 +330,7 @@ int ltca_kv8_decode_workspace_bytes(const ltca_kv8_cache* c, const ltca_kv8_deco
 typedef struct {
     int32_t Hq, Sq;
     int32_t dtype;              /* ltca_dtype of q                                   */
-    const void* q; ltca_strides q_strides;     /* [B,Hq,Sq,D], any alignment         */
+    const void* q; ltca_strides q_strides;     /* [B,Hq,Sq,D], rows on any element   */
     const int32_t* kv_len;      /* optional [B], with the new tokens; NULL: all S    */
     const int32_t* new_len;     /* optional [B] (0 .. Sq): rows that count (none: all scores are equal); NULL: Sq */
     int32_t first, last;        /* each >= 0, first + last <= count                  */
